@@ -523,6 +523,67 @@ int pv_dropout_f32(const float* src, int n0, int n1, int C, long s0, long s1, lo
 int pv_dropout_pack_bf16(const float* src, int n0, int n1, int n1p, int C, long s0, long s1, long sc, long m0, long m1,
                          float p, const void* mask, const void* rng_state, int site, void* dst, int ldd, void* stream);
 
+/* ---- losses over rows of a vocabulary softmax in memory -------------------------------------------------------
+ * No counterpart in the reference, whose losses stop at the NLL of a given text (criterions.py:24-138): what a decoder
+ * learns from another model's answers and from judgments of its own samples (decoders.py:255-256) starts at the
+ * log-probabilities below.
+ * logits: [n0][n1] rows of V words, words contiguous, rows at any element stride (s0, s1) and any element address, dtype
+ * PV_DTYPE_*; log-probabilities serve as logits.  inv_temp: 1 / temperature.  tokens / labels: int64 [n0 * n1]; rows whose
+ * entry is `ignore` are dead: not read, zero in every output.  A live entry outside [0, V) makes its row's outputs NaN, and
+ * so does a row without a finite logit.  Limits: 2^31 - 1 rows, 2^24 words (PV_ERR_LIMIT).
+ * Gradients (dlogits) are contiguous [n0 * n1][V] of the logits' type.  `save`: 4 floats a row, handed from the forward to
+ * the backward call (NULL: no gradient wanted).  ws: pv_vocab_rows_ws_bytes(rows). */
+#define PV_DTYPE_F32 0
+#define PV_DTYPE_BF16 1
+#define PV_DTYPE_F16 2
+size_t pv_vocab_rows_ws_bytes(long rows);
+/* logp[t] = log_softmax(logits * inv_temp)[t][tokens[t]]; entropy[t] (NULL: not wanted) of the same distribution.  Backward
+ * for upstream gradients dlogp / dentropy [rows] (either may be NULL). */
+int pv_token_logp_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                      int64_t ignore, float inv_temp, float* logp, float* entropy, float* save, void* stream);
+int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                      int64_t ignore, float inv_temp, const float* save, const float* dlogp, const float* dentropy,
+                      void* dlogits, void* stream);
+/* Clipped policy loss of sampled tokens, with r = exp(logp - old_logp) and d = ref_logp - logp:
+ *   loss = scale * sum over live rows of [ -min(r A, clip(r, clip_lo, clip_hi) A) + kl_coef (e^d - 1 - d) - ent_coef H ]
+ * scale = weight, or weight / (live rows, at least 1) with word != 0.  ref_logp NULL: no KL term.  adv: [n0 * n1] with
+ * adv_per_token, else [n0].  stats[4]: means over live rows of the policy term, of the KL term, of "the clip decides" and of
+ * H.  Backward: g = upstream gradient of the loss (device scalar). */
+int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                       int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
+                       int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
+                       float* loss, float* stats, float* save, void* ws, void* stream);
+int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                       int64_t ignore, float inv_temp, const float* save, const float* g, void* dlogits, void* stream);
+/* Distillation from a teacher's K top logits (t_ids int64 / t_logits [rows][K], K <= pv_distill_max_entries()): with p the
+ * softmax of the row's teacher logits and q that of its logits, both at the temperature 1 / inv_temp,
+ *   loss = scale / inv_temp^2 * sum over live rows of sum_j p_j (log p_j - log q[t_ids_j])
+ * Entries of -inf do not count (their ids are not read as words); a row without any counts as dead except for the live count.
+ * labels NULL: every row is live.  psum: [rows][K] floats kept for the backward call. */
+int pv_distill_max_entries(void);
+int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
+                        int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
+                        float weight, int word, float* loss, float* save, float* psum, void* ws, void* stream);
+int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp,
+                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, void* dlogits,
+                        void* stream);
+/* The same policy loss from log-probabilities (no entropy term, stats[3] = 0).  dlogp: n0 * n1 + 1 floats kept for the backward
+ * call (the last one is the scale; NULL: no gradient wanted).  ws: pv_vocab_rows_ws_bytes(0). */
+int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,
+                         const float* ref_logp, const float* adv, int adv_per_token, float clip_lo, float clip_hi,
+                         float kl_coef, float weight, int word, float* loss, float* stats, float* dlogp, void* ws,
+                         void* stream);
+int pv_policy_tokens_bwd(const float* dlogp, const float* g, long n, float* d, void* stream);
+/* Preference loss over pairs of answers from their tokens' log-probabilities [pairs][Lc] / [pairs][Lr] and a reference
+ * model's (NULL: none): rewards = beta * sum over live tokens of (logp - ref), chosen [pairs] then rejected [pairs],
+ * x = their difference, loss = weight * sum over pairs of [ -(1 - smoothing) ln sig(x) - smoothing ln sig(-x) ].
+ * slope: [pairs] kept for the backward call; ws: pv_vocab_rows_ws_bytes(pairs). */
+int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* labels_c, int Lc, const float* logp_r,
+                      const float* ref_r, const int64_t* labels_r, int Lr, long pairs, int64_t ignore, float beta,
+                      float smoothing, float weight, float* loss, float* rewards, float* slope, void* ws, void* stream);
+int pv_preference_bwd(const int64_t* labels_c, int Lc, const int64_t* labels_r, int Lr, long pairs, int64_t ignore,
+                      const float* slope, float weight, const float* g, float* dlogp_c, float* dlogp_r, void* stream);
+
 /* ---- clip + skip guards + Adam over one flat buffer (main_pretrain.py:207-225,268-269;
  * dialog_models.py:122-131) ------------------------------------------------------------------------------------ */
 /* state: pv_optim_state_bytes() of device memory, zeroed once; its first 48 bytes are {float avg_norm; int have_avg,

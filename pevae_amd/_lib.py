@@ -32,6 +32,8 @@ class BlockCall(C.Structure):
 
 BLOCK_GROUP_MAX = 3
 
+_ROWS = [vp, i32, lng, i32, lng, lng, i32]      # logits, dtype, n0, n1, s0, s1, V of the losses over rows in memory
+
 # name -> (restype, argtypes); mirrors include/pevae_hip.h one-to-one (tests/test_abi.py checks that)
 SIGNATURES = {
     "pv_last_error": (C.c_char_p, []),
@@ -145,6 +147,18 @@ SIGNATURES = {
     "pv_rng_advance": (i32, [vp, vp]),
     "pv_dropout_f32": (i32, [vp, i32, i32, i32, lng, lng, lng, lng, lng, f32, vp, vp, i32, vp, lng, lng, vp]),
     "pv_dropout_pack_bf16": (i32, [vp, i32, i32, i32, i32, lng, lng, lng, lng, lng, f32, vp, vp, i32, vp, i32, vp]),
+    "pv_vocab_rows_ws_bytes": (sz, [lng]),
+    "pv_token_logp_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp]),
+    "pv_token_logp_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp, vp]),
+    "pv_policy_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, i32, f32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),
+    "pv_policy_rows_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp]),
+    "pv_distill_max_entries": (i32, []),
+    "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp]),
+    "pv_distill_rows_bwd": (i32, _ROWS + [f32, vp, i32, vp, vp, vp, vp, vp]),
+    "pv_policy_tokens_fwd": (i32, [vp, vp, i64, lng, i32, vp, vp, vp, i32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),
+    "pv_policy_tokens_bwd": (i32, [vp, vp, lng, vp, vp]),
+    "pv_preference_fwd": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, lng, i64, f32, f32, f32, vp, vp, vp, vp, vp]),
+    "pv_preference_bwd": (i32, [vp, i32, vp, i32, lng, i64, vp, f32, vp, vp, vp, vp]),
     "pv_optim_state_bytes": (sz, []),
     "pv_grad_guard": (i32, [vp, lng, vp, f32, f32, i32, f32, f32, i32, f32, vp]),
     "pv_adam_step": (i32, [vp, vp, vp, vp, lng, vp, f32, f32, f32, f32, vp]),

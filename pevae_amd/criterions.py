@@ -106,3 +106,76 @@ class Entropy(_Loss):
         if unit_average:
             return ops.mean(h_q)
         return ops.sum(h_q) / batch_size
+
+
+# ------------------------------------------------------------------------------------------------------------
+# Learning from another model's answers and from judgments of one's own: no counterpart in the reference.  Like the losses
+# above they take a dense [B, L, V] tensor (log-probabilities or logits, fp32 / bf16 / fp16) or the decoder's DeferredLogProbs.
+# ------------------------------------------------------------------------------------------------------------
+
+def token_log_probs(net_output, labels, padding_idx):
+    """Log-probability of `labels` [B, L] per token (fp32 [B, L], differentiable; 0 at padding): what the policy and preference
+    losses ask of the old policy and of a reference model, under torch.no_grad()."""
+    if isinstance(net_output, DeferredLogProbs):
+        return net_output.token_logp(labels, padding_idx)
+    return ops.token_logprobs(net_output, labels, ignore_index=padding_idx)
+
+
+class TopKDistill(_Loss):
+    """Distillation from a teacher's top logits (ops.distill_topk): forward(net_output, labels, teacher_ids, teacher_logits)
+    with teacher_ids / teacher_logits [B, L, K] -> loss.  avg_type as NLLEntropy's: 'seq' = sum / batch, 'word' = token mean,
+    None = sum.  A DeferredLogProbs is materialised: the teacher's softmax needs the whole row's statistics and K words of it."""
+
+    def __init__(self, padding_idx, config, temperature=1.0, weight=1.0, avg_type="seq"):
+        super().__init__()
+        if avg_type not in ("word", "seq", None):
+            raise NotImplementedError("Unknown avg type")
+        self.padding_idx, self.temperature, self.weight, self.avg_type = padding_idx, temperature, weight, avg_type
+
+    def forward(self, net_output, labels, teacher_ids, teacher_logits):
+        if isinstance(net_output, DeferredLogProbs):
+            net_output = net_output.materialize()
+        return ops.distill_topk(net_output, teacher_ids, teacher_logits, labels, self.padding_idx, self.temperature,
+                                self.weight, self.avg_type)
+
+
+class ClippedPolicyLoss(_Loss):
+    """Clipped policy loss with a KL term and an entropy bonus (ops.vocab_policy_loss): forward(net_output, labels, old_logp,
+    advantages, ref_logp=None) -> (loss, stats), labels = the sampled tokens [B, L], padded.  A DeferredLogProbs goes through
+    the fused vocabulary projection (no [B, L, V] tensor) unless there is an entropy bonus, which needs the rows."""
+
+    def __init__(self, padding_idx, config, clip=0.2, clip_high=None, kl_coef=0.0, ent_coef=0.0, weight=1.0, avg_type="word"):
+        super().__init__()
+        if avg_type not in ("word", "seq", None):
+            raise NotImplementedError("Unknown avg type")
+        self.padding_idx, self.clip, self.clip_high = padding_idx, clip, clip_high
+        self.kl_coef, self.ent_coef, self.weight, self.avg_type = kl_coef, ent_coef, weight, avg_type
+
+    def forward(self, net_output, labels, old_logp, advantages, ref_logp=None):
+        if isinstance(net_output, DeferredLogProbs):
+            if self.ent_coef == 0:
+                return ops.policy_loss(net_output.token_logp(labels, self.padding_idx), labels, old_logp, advantages, ref_logp,
+                                       self.padding_idx, self.clip, self.clip_high, self.kl_coef, self.weight, self.avg_type)
+            net_output = net_output.materialize()
+        return ops.vocab_policy_loss(net_output, labels, old_logp, advantages, ref_logp, self.padding_idx, 1.0, self.clip,
+                                     self.clip_high, self.kl_coef, self.ent_coef, self.weight, self.avg_type)
+
+
+class PreferenceLoss(_Loss):
+    """Preference loss over pairs of answers (ops.preference_loss): forward(chosen_output, chosen_labels, rejected_output,
+    rejected_labels, ref_chosen=None, ref_rejected=None) -> (loss, chosen rewards, rejected rewards).  The outputs are those
+    of the decoder for the two answers; ref_*: the reference model's token_log_probs.  avg_type: 'seq' = mean over pairs,
+    None = sum."""
+
+    def __init__(self, padding_idx, config, beta=0.1, label_smoothing=0.0, weight=1.0, avg_type="seq"):
+        super().__init__()
+        if avg_type not in ("seq", None):
+            raise NotImplementedError("Unknown avg type")
+        self.padding_idx, self.beta, self.label_smoothing = padding_idx, beta, label_smoothing
+        self.weight, self.avg_type = weight, avg_type
+
+    def forward(self, chosen_output, chosen_labels, rejected_output, rejected_labels, ref_chosen=None, ref_rejected=None):
+        return ops.preference_loss(token_log_probs(chosen_output, chosen_labels, self.padding_idx), chosen_labels,
+                                   token_log_probs(rejected_output, rejected_labels, self.padding_idx), rejected_labels,
+                                   ref_chosen, ref_rejected, self.padding_idx, self.beta, self.label_smoothing, self.weight,
+                                   self.avg_type)

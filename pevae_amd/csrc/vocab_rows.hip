@@ -1,0 +1,887 @@
+// Losses over rows of a vocabulary softmax held in memory ([T][V] logits or log-probabilities, fp32 / bf16 / fp16), next to
+// the NLL of a given text: per-token log-probability and entropy, distillation from a teacher's top logits, the clipped
+// policy loss with a KL term, and the preference loss over pairs of answers, each with its gradient.
+//
+// With c = 1 / temperature, m = max_v z_v, s = sum_v exp(c (z_v - m)), p_v = exp(c (z_v - m)) / s:
+//   log p_v = c (z_v - m) - ln s,   H = ln s - sum_v p_v c (z_v - m)
+// and every gradient has the form  dz_v = e_v (a + b x_v) + [v in a short list] d_v,  x_v = c log2(e) (z_v - m), e_v = 2^x_v,
+// with a, b and the list known once the row's statistics are.  All statistics, sums and coefficients are fp32 or fp64;
+// only the gradient is rounded to the logits' type, once.
+//
+// The rows are read in 16-byte pieces whatever the address of a row is (odd vocabularies put rows at any element):
+// gfx950 takes unaligned global accesses.
+#include "common.h"
+#include "../../include/pevae_hip.h"
+
+namespace {
+
+constexpr int kTeacherMax = 256;        // teacher entries a row: four a lane of one wave
+constexpr int kVocabMax = 1 << 24;      // indices of a row fit fp32 and int32 with room
+constexpr float kFloorX = -2.0e4f;      // 2^kFloorX is 0: keeps 0 * (-inf) out of the entropy terms
+constexpr float kDead = __builtin_inff();   // `m` of a row that is not computed (padding, empty teacher list)
+
+enum { HEAD_TOKEN = 0, HEAD_POLICY = 1, HEAD_DISTILL = 2 };
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(1))) piece_t { u32x4 v; };     // 16 bytes at any address
+
+// (a copy of the element: __builtin_bit_cast of an element of a vector register reads element 0)
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_uint(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+struct F32 {
+  typedef float type;
+  static constexpr int N = 4;
+  static __device__ __forceinline__ float up(float x) { return x; }
+  static __device__ __forceinline__ float down(float x) { return x; }
+  static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = as_float(r[i]);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = as_uint(f[i]);
+    return r;
+  }
+};
+struct BF16 {
+  typedef bf16_t type;
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float up(bf16_t x) { return bf2f(x); }
+  static __device__ __forceinline__ bf16_t down(float x) { return f2bf(x); }
+  static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = as_float(r[i] << 16);
+      f[2 * i + 1] = as_float(r[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2bf(f[2 * i], f[2 * i + 1]);
+    return r;
+  }
+};
+struct F16 {
+  typedef uint16_t type;
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float up(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+  static __device__ __forceinline__ uint16_t down(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+  static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = up((uint16_t)(r[i] & 0xffffu));
+      f[2 * i + 1] = up((uint16_t)(r[i] >> 16));
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (uint32_t)down(f[2 * i]) | ((uint32_t)down(f[2 * i + 1]) << 16);
+    return r;
+  }
+};
+
+__device__ __forceinline__ u32x4 load_piece(const void* p) { return ((const piece_t*)p)->v; }
+__device__ __forceinline__ void store_piece(void* p, u32x4 v) { ((piece_t*)p)->v = v; }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// Softmax statistics of a part of a row: maximum, sum of e = 2^x, sum of e x (x in units of log2).  An empty part is
+// {-inf, 0, 0}; a NaN among the elements makes s NaN (fmaxf alone would drop it).
+struct Stat {
+  float m, s, ex;
+};
+__device__ __forceinline__ float finite_max(float m) { return m == -__builtin_inff() ? 0.f : m; }
+// the part seen from the maximum mm >= st.m (finite, or +inf / NaN that the result carries on)
+__device__ __forceinline__ void rebase(Stat& st, float mm, float k) {
+  const float d = (st.m - mm) * k, f = exp2_(d);
+  st.ex = (st.ex + st.s * fmaxf(d, kFloorX)) * f;
+  st.s *= f;
+}
+__device__ __forceinline__ Stat wave_stat(Stat st, float k) {
+  const float m = wave_max(st.m);
+  rebase(st, finite_max(m), k);
+  return {m, wave_sum(st.s), wave_sum(st.ex)};
+}
+
+// x - ln(s) to about half a unit of the result: ln s = n ln2 + ln f with the two halves of ln2 kept apart, the rounding of
+// the first difference carried into the second.
+__device__ __forceinline__ float minus_log(float x, float s) {
+  if (!(fabsf(x) < __builtin_inff()) || !(s > 0.f && s < __builtin_inff())) return x - logf(s);
+  int n;
+  float f = frexpf(s, &n);
+  if (f < 0.70710678f) {
+    f *= 2.f;
+    n -= 1;
+  }
+  const float hi = (float)n * 0.693145751953125f;                  // 16 bits of ln2: exact times n
+  const float lo = (float)n * 1.42860682e-6f + logf(f);
+  const float t = x - hi, bb = t - x;
+  const float err = (x - (t - bb)) + (-hi - bb);
+  return t + (err - lo);
+}
+// e^d - 1 - d; its leading terms cancel for small d
+__device__ __forceinline__ float exp_minus_1_minus(float d, float em1) {
+  if (fabsf(d) >= 0.25f) return em1 - d;
+  return d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040))))));
+}
+
+// ---- arguments ---------------------------------------------------------------------------------------------------------
+struct Rows {
+  const void* logits;
+  int n1, V;                 // row t = (t / n1, t % n1)
+  long T, s0, s1;            // element strides of the two row indices
+  float c, k;                // 1 / temperature, c * log2(e)
+  const int64_t* labels;     // NULL: every row is live and there is no label
+  int64_t ignore;
+};
+struct Policy {
+  const float *old_lp, *ref_lp, *adv;      // ref_lp NULL: no KL term; adv [T] or [T / n1]
+  int adv_per_row;
+  float lo, hi, kl, ent;
+};
+struct Distill {
+  const int64_t* ids;        // [T][K]
+  const void* t_logits;      // [T][K]
+  int K, dtype;
+  float* psum;               // [T][K]: the teacher's probability of the entry's word, duplicates added up
+};
+struct Scale {
+  float weight;              // of the loss, divided by *count where count != NULL (at least 1)
+  const float* count;
+  __device__ __forceinline__ float get() const { return count ? weight / fmaxf(*count, 1.f) : weight; }
+};
+
+template <class E>
+__device__ __forceinline__ const typename E::type* row_of(const Rows& a, long t) {
+  const uint32_t i = (uint32_t)t / (uint32_t)a.n1, j = (uint32_t)t - i * (uint32_t)a.n1;     // fewer than 2^31 rows
+  return (const typename E::type*)a.logits + i * a.s0 + j * a.s1;
+}
+
+struct PolicyTerm {
+  float pg, k3, cut, dlp;
+};
+// -min(r A, clip(r) A) with r = exp(lp - old), and kl times the estimate e^d - 1 - d, d = ref - lp, of the divergence
+__device__ __forceinline__ PolicyTerm policy_term(const Policy& h, float lp, float old_lp, float ref_lp, float A) {
+  const float r = expf(lp - old_lp);
+  float u = r * A, w = fminf(fmaxf(r, h.lo), h.hi) * A;
+  if (A == 0.f) u = w = 0.f;                      // r may be infinite
+  PolicyTerm o;
+  const bool cut = u > w;
+  o.cut = cut ? 1.f : 0.f;
+  o.pg = cut ? -w : -u;
+  o.dlp = cut ? 0.f : -u;
+  o.k3 = 0.f;
+  if (h.ref_lp) {
+    const float d = ref_lp - lp, em1 = expm1f(d);
+    o.k3 = exp_minus_1_minus(d, em1);
+    o.dlp -= h.kl * em1;
+  }
+  return o;
+}
+
+__device__ __forceinline__ float load_teacher(const Distill& h, long i) {
+  if (h.dtype == PV_DTYPE_F32) return ((const float*)h.t_logits)[i];
+  const uint16_t v = ((const uint16_t*)h.t_logits)[i];
+  return h.dtype == PV_DTYPE_BF16 ? bf2f(v) : (float)__builtin_bit_cast(_Float16, v);
+}
+
+// The teacher's side of a row, by one wave: its softmax over the K entries (those of -inf do not count), the sum of
+// p (log p - c (z - zref)) over the entries, and for each entry the probability of its word (duplicate words added up).
+// empty: no entry counts.  bad: an entry that counts names a word outside the vocabulary.
+struct Teacher {
+  float acc, zref;
+  bool empty, bad;
+};
+template <class E>
+__device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, long t, const typename E::type* row, int lane) {
+  float x[4], z[4], p[4];
+  int id[4];
+  float mx = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = lane + 64 * i;
+    x[i] = -__builtin_inff();
+    id[i] = -1;
+    if (j < h.K) {
+      x[i] = load_teacher(h, t * h.K + j);
+      const int64_t w = h.ids[t * h.K + j];
+      id[i] = w >= 0 && w < a.V ? (int)w : -1;
+    }
+    mx = fmaxf(mx, x[i]);
+  }
+  float nan = 0.f;                                 // fmaxf drops a NaN: the sum below keeps it
+#pragma unroll
+  for (int i = 0; i < 4; ++i) nan += x[i] != x[i] ? x[i] : 0.f;
+  mx = wave_max(mx) + wave_sum(nan);
+  Teacher r;
+  r.empty = mx == -__builtin_inff();
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    z[i] = id[i] >= 0 ? E::up(row[id[i]]) : 0.f;
+    p[i] = x[i] == -__builtin_inff() ? 0.f : exp2_((x[i] - mx) * a.k);
+    sum += p[i];
+  }
+  sum = wave_sum(sum);
+  const float inv = r.empty ? 0.f : 1.f / sum;
+  float zr = -__builtin_inff(), bad = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[i] *= inv;
+    if (p[i] > 0.f) {
+      if (id[i] < 0) bad = 1.f;
+      zr = fmaxf(zr, z[i]);
+    }
+  }
+  r.bad = wave_sum(bad) > 0.f || sum != sum;       // (a NaN or +inf among the teacher's logits)
+  r.zref = finite_max(wave_max(zr));
+  float acc = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p[i] > 0.f) acc += p[i] * (minus_log((x[i] - mx) * a.c, sum) - a.c * (z[i] - r.zref));
+  r.acc = wave_sum(acc);
+  float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int n = h.K - 64 * q < 64 ? h.K - 64 * q : 64;
+    for (int l = 0; l < n; ++l) {
+      const int w = __shfl(id[q], l);
+      const float pw = __shfl(p[q], l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ps[i] += w == id[i] ? pw : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 64 * i < h.K) h.psum[t * h.K + lane + 64 * i] = ps[i];
+  return r;
+}
+
+// ---- forward: statistics and losses of a row, one workgroup each ---------------------------------------------------------
+struct FwdOut {
+  float *logp, *ent;         // HEAD_TOKEN
+  float4* rowout;            // HEAD_POLICY {pg, k3, cut, H}, HEAD_DISTILL {loss, -, -, -} of the row, unscaled
+  float4* save;              // what the gradient pass starts from: HEAD_TOKEN {m, 1/s, ex/s, -}, else {m, a, b, d}
+};
+
+// running statistics of a thread over n elements held in registers (-inf where there is none)
+template <int N, bool ENT>
+__device__ __forceinline__ void accumulate(Stat& st, const float (&z)[N], float k) {
+  float mb = z[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mb = fmaxf(mb, z[i]);
+  const float m = fmaxf(st.m, mb), mm = finite_max(m);
+  const float d = (st.m - mm) * k, f = exp2_(d);
+  float s = st.s * f, ex = ENT ? (st.ex + st.s * fmaxf(d, kFloorX)) * f : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = (z[i] - mm) * k, e = exp2_(x);
+    s += e;
+    if (ENT) ex += e * fmaxf(x, kFloorX);
+  }
+  st = {m, s, ex};
+}
+
+// the row's loss terms and the coefficients of its gradient
+template <int HEAD>
+__device__ __forceinline__ void finish_row(const Rows& a, const Policy& hp, const Scale& sc, const Teacher& te, const FwdOut& o,
+                                           long t, Stat st, float zy, bool bad) {
+  const float nan = __builtin_nanf("");
+  const float inv = 1.f / st.s, ln2 = 0.69314718056f;
+  if (st.m == kDead) st.m = nan;                   // a logit of +inf: no distribution
+  if (HEAD == HEAD_TOKEN) {
+    const float H = -minus_log(st.ex * inv * ln2, st.s);
+    if (o.logp) o.logp[t] = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
+    if (o.ent) o.ent[t] = H;
+    if (o.save) o.save[t] = make_float4(bad ? nan : st.m, inv, st.ex * inv, 0.f);
+  } else if (HEAD == HEAD_POLICY) {
+    const float lp = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
+    const float H = -minus_log(st.ex * inv * ln2, st.s);
+    const PolicyTerm q = policy_term(hp, lp, hp.old_lp[t], hp.ref_lp ? hp.ref_lp[t] : 0.f, hp.adv[hp.adv_per_row ? t : (long)((uint32_t)t / (uint32_t)a.n1)]);
+    o.rowout[t] = make_float4(q.pg, q.k3, q.cut, H);
+    if (o.save) {
+      // d(loss)/d(log p[y]) = g, d(loss)/dH = h: dz_v = c (g [v = y] - p_v (g + h (log p_v + H)))
+      const float w = sc.get(), g = w * q.dlp, h = -w * hp.ent;
+      o.save[t] = make_float4(st.m, -a.c * inv * (g - h * ln2 * st.ex * inv), -a.c * inv * h * ln2, a.c * g);
+    }
+  } else {
+    const float tau = 1.f / a.c;
+    const float loss = te.bad ? nan : te.acc + (a.c * (st.m - te.zref) - minus_log(0.f, st.s));
+    o.rowout[t] = make_float4(te.empty ? 0.f : tau * tau * loss, 0.f, 0.f, 0.f);
+    if (o.save) {
+      const float w = sc.get() * tau;             // tau^2 / tau
+      o.save[t] = make_float4(te.empty ? kDead : st.m, te.bad ? nan : w * inv, 0.f, -w);
+    }
+  }
+}
+
+template <class E, int HEAD, bool ENT>
+__global__ __launch_bounds__(256) void rows_fwd_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o) {
+  const long t = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t y = a.labels ? a.labels[t] : -1;
+  if (a.labels && y == a.ignore) {
+    if (tid == 0) {
+      if (HEAD == HEAD_TOKEN) {
+        if (o.logp) o.logp[t] = 0.f;
+        if (o.ent) o.ent[t] = 0.f;
+      } else {
+        o.rowout[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (o.save) o.save[t] = make_float4(kDead, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
+  const typename E::type* row = row_of<E>(a, t);
+  const bool bad = HEAD != HEAD_DISTILL && (y < 0 || y >= a.V);
+  const float zy = HEAD != HEAD_DISTILL && !bad ? E::up(row[y]) : 0.f;
+  Teacher te = {0.f, 0.f, false, false};
+  if (HEAD == HEAD_DISTILL && wave == 0) te = teacher_row<E>(a, hd, t, row, lane);
+  Stat st = {-__builtin_inff(), 0.f, 0.f};
+  const int full = a.V / E::N;
+  for (int c0 = tid; c0 < full; c0 += 4 * 256) {
+    u32x4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + i * 256 < full) raw[i] = load_piece(row + (long)(c0 + i * 256) * E::N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + i * 256 < full) {
+        float z[E::N];
+        E::unpack(raw[i], z);
+        accumulate<E::N, ENT>(st, z, a.k);
+      }
+  }
+  const int rest = full * E::N + tid;
+  if (rest < a.V) {
+    float z[1] = {E::up(row[rest])};
+    accumulate<1, ENT>(st, z, a.k);
+  }
+  st = wave_stat(st, a.k);
+  __shared__ Stat part[4];
+  if (lane == 0) part[wave] = st;
+  __syncthreads();
+  if (wave != 0) return;
+  st = lane < 4 ? part[lane] : Stat{-__builtin_inff(), 0.f, 0.f};
+  st = wave_stat(st, a.k);
+  if (lane == 0) finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad);
+}
+
+// ---- gradient: dz_v = g (e_v (a + b x_v) + d [v in the row's list]), pieces of rows dealt out to workgroups ----------------
+struct Grad {
+  const float4* save;
+  const float *dlogp, *dent; // HEAD_TOKEN: upstream gradients a row
+  const float* g;            // else: upstream gradient of the loss (device scalar)
+  void* out;                 // [T][V]
+};
+
+template <class E, int HEAD>
+__global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad q, int blocks_per_row, long items) {
+  const int tid = threadIdx.x;
+  constexpr int kItem = 256 * 4 * E::N;            // elements of a row that a workgroup takes at a time
+  const float up = HEAD == HEAD_TOKEN ? 1.f : *q.g;
+  for (long it = blockIdx.x; it < items; it += gridDim.x) {
+    const long t = it / blocks_per_row;
+    const int v0 = (int)(it - t * blocks_per_row) * kItem, v1 = a.V - v0 < kItem ? a.V : v0 + kItem;
+    typename E::type* out = (typename E::type*)q.out + t * a.V;
+    const int full = (v1 - v0) / E::N;             // a multiple of the piece except at the row's end
+    float4 w = q.save[t];
+    float dy = 0.f;
+    int y = -1;
+    if (HEAD == HEAD_TOKEN) {
+      const float g = q.dlogp ? q.dlogp[t] : 0.f, h = q.dent ? q.dent[t] : 0.f, ln2 = 0.69314718056f;
+      if (w.x != kDead) {
+        w = make_float4(w.x, -a.c * w.y * (g - h * ln2 * w.z), -a.c * w.y * h * ln2, 0.f);
+        dy = a.c * g;
+        y = (int)a.labels[t];
+      }
+    } else {
+      w.y *= up;
+      w.z *= up;
+      dy = w.w * up;
+      if (HEAD == HEAD_POLICY && w.x != kDead) y = (int)a.labels[t];
+    }
+    if (w.x == kDead) {
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+      for (int i = tid; i < full; i += 256) store_piece(out + v0 + (long)i * E::N, zero);
+      if (v0 + full * E::N + tid < v1) out[v0 + full * E::N + tid] = E::down(0.f);
+      continue;
+    }
+    const typename E::type* row = row_of<E>(a, t);
+    u32x4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (tid + i * 256 < full) raw[i] = load_piece(row + v0 + (long)(tid + i * 256) * E::N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (tid + i * 256 >= full) break;
+      const int v = v0 + (tid + i * 256) * E::N;
+      float z[E::N];
+      E::unpack(raw[i], z);
+#pragma unroll
+      for (int n = 0; n < E::N; ++n) {
+        const float x = (z[n] - w.x) * a.k, e = exp2_(x);
+        z[n] = w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
+        if (HEAD != HEAD_DISTILL && v + n == y) z[n] += dy;
+      }
+      store_piece(out + v, E::pack(z));
+    }
+    const int rest = v0 + full * E::N + tid;
+    if (rest < v1) {
+      const float x = (E::up(row[rest]) - w.x) * a.k, e = exp2_(x);
+      float d = w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
+      if (HEAD != HEAD_DISTILL && rest == y) d += dy;
+      out[rest] = E::down(d);
+    }
+    if (HEAD == HEAD_DISTILL) {
+      __syncthreads();                             // the list's words are written again, after the sweep
+      if (tid < hd.K) {
+        const int64_t id = hd.ids[t * hd.K + tid];
+        if (id >= v0 && id < v1) {
+          const float e = exp2_((E::up(row[id]) - w.x) * a.k);
+          out[id] = E::down(e * w.y + dy * hd.psum[t * hd.K + tid]);
+        }
+      }
+    }
+  }
+}
+
+// ---- sums --------------------------------------------------------------------------------------------------------------
+// Fixed order: a workgroup's threads take rows a stride apart, its tree is fixed, a second launch adds the workgroups' sums.
+struct Sum5 {
+  double v[5];
+};
+__device__ __forceinline__ void block_sum(double (&v)[5], double (*sh)[5]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    v[i] = wave_sum(v[i]);
+    if (lane == 0) sh[wave][i] = v[i];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 0; i < 5; ++i) {
+      v[i] = sh[0][i];
+      for (int w = 1; w < waves; ++w) v[i] += sh[w][i];
+    }
+}
+// what becomes of the sums of {pg, k3, cut, H, live}
+struct Result {
+  float kl, ent, weight;
+  int word;
+  float* loss;
+  float* stats;              // [4] means over live rows; NULL: not wanted
+  float* scale;              // what the rows' terms were multiplied by; NULL: not wanted
+};
+__device__ __forceinline__ void write_result(const double (&v)[5], const Result& r) {
+  const double n = v[4] > 1.0 ? v[4] : 1.0;
+  const double scale = r.word ? r.weight / n : r.weight;
+  *r.loss = (float)(scale * (v[0] + (double)r.kl * v[1] - (double)r.ent * v[3]));
+  if (r.stats)
+    for (int i = 0; i < 4; ++i) r.stats[i] = (float)(v[i] / n);
+  if (r.scale) *r.scale = (float)scale;
+}
+
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const float4* __restrict__ rows, const int64_t* __restrict__ labels,
+                                                        int64_t ignore, long T, Sum5* __restrict__ part, Result r) {
+  __shared__ double sh[16][5];
+  double v[5] = {0, 0, 0, 0, 0};
+  for (long t = blockIdx.x * 1024L + threadIdx.x; t < T; t += gridDim.x * 1024L) {
+    const float4 q = rows[t];
+    v[0] += q.x;
+    v[1] += q.y;
+    v[2] += q.z;
+    v[3] += q.w;
+    v[4] += !labels || labels[t] != ignore ? 1.0 : 0.0;
+  }
+  block_sum(v, sh);
+  if (threadIdx.x == 0) {
+    if (gridDim.x > 1) {
+      for (int i = 0; i < 5; ++i) part[blockIdx.x].v[i] = v[i];
+    } else {
+      write_result(v, r);
+    }
+  }
+}
+__global__ __launch_bounds__(256) void sum_parts_kernel(const Sum5* __restrict__ part, int n, Result r) {
+  __shared__ double sh[16][5];
+  double v[5] = {0, 0, 0, 0, 0};
+  for (int t = threadIdx.x; t < n; t += 256)
+    for (int i = 0; i < 5; ++i) v[i] += part[t].v[i];
+  block_sum(v, sh);
+  if (threadIdx.x == 0) write_result(v, r);
+}
+constexpr int kSumGroups = 256;
+inline int sum_groups(long T) {
+  const long g = (T + 16383) / 16384;
+  return (int)(g < 1 ? 1 : g > kSumGroups ? kSumGroups : g);
+}
+
+// live rows, before a pass that divides by them
+__global__ __launch_bounds__(1024) void count_live_kernel(const int64_t* __restrict__ labels, int64_t ignore, long T,
+                                                          float* __restrict__ part, float* __restrict__ out) {
+  __shared__ int sh[16];
+  int n = 0;
+  for (long t = blockIdx.x * 1024L + threadIdx.x; t < T; t += gridDim.x * 1024L) n += labels[t] != ignore ? 1 : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) n += sh[w];
+    (gridDim.x > 1 ? part[blockIdx.x] : out[0]) = (float)n;
+  }
+}
+__global__ __launch_bounds__(256) void add_counts_kernel(const float* __restrict__ part, int n, float* __restrict__ out) {
+  __shared__ double sh[16][5];
+  double v[5] = {(int)threadIdx.x < n ? (double)part[threadIdx.x] : 0.0, 0, 0, 0, 0};
+  block_sum(v, sh);
+  if (threadIdx.x == 0) out[0] = (float)v[0];
+}
+
+// ---- policy loss from log-probabilities ------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void policy_tokens_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels,
+                                                            int64_t ignore, long T, int n1, Policy h, float* __restrict__ dlp,
+                                                            Sum5* __restrict__ part, Result r) {
+  __shared__ double sh[16][5];
+  double v[5] = {0, 0, 0, 0, 0};
+  for (long t = blockIdx.x * 256L + threadIdx.x; t < T; t += gridDim.x * 256L) {
+    float d = 0.f;
+    if (labels[t] != ignore) {
+      const PolicyTerm q = policy_term(h, logp[t], h.old_lp[t], h.ref_lp ? h.ref_lp[t] : 0.f, h.adv[h.adv_per_row ? t : t / n1]);
+      v[0] += q.pg;
+      v[1] += q.k3;
+      v[2] += q.cut;
+      v[4] += 1.0;
+      d = q.dlp;
+    }
+    if (dlp) dlp[t] = d;
+  }
+  block_sum(v, sh);
+  if (threadIdx.x == 0) {
+    if (gridDim.x > 1) {
+      for (int i = 0; i < 5; ++i) part[blockIdx.x].v[i] = v[i];
+    } else {
+      write_result(v, r);
+    }
+  }
+}
+// d logp = g * scale * dlp
+__global__ __launch_bounds__(256) void policy_tokens_bwd_kernel(const float* __restrict__ dlp, const float* __restrict__ scale,
+                                                                const float* __restrict__ g, long T, float* __restrict__ out) {
+  const float w = *g * *scale;
+  for (long t = blockIdx.x * 256L + threadIdx.x; t < T; t += gridDim.x * 256L) out[t] = w * dlp[t];
+}
+
+// ---- preference loss -----------------------------------------------------------------------------------------------------
+struct Answers {
+  const float *logp, *ref;   // [P][L]; ref NULL: no reference model
+  const int64_t* labels;
+  int L;
+};
+// sum over the live tokens of (log p - log p_ref), in fp64: long answers cancel
+__device__ __forceinline__ double answer_sum(const Answers& a, int64_t ignore, long b) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < a.L; i += 256) {
+    const long t = b * a.L + i;
+    if (a.labels[t] != ignore) v += (double)a.logp[t] - (a.ref ? (double)a.ref[t] : 0.0);
+  }
+  return v;
+}
+// One workgroup a pair: x = beta (sum_chosen - sum_rejected), loss = -(1 - e) ln sig(x) - e ln sig(-x), its slope.
+__global__ __launch_bounds__(256) void preference_kernel(Answers c, Answers r, int64_t ignore, float beta, float smooth,
+                                                         float* __restrict__ reward_c, float* __restrict__ reward_r,
+                                                         float* __restrict__ slope, float4* __restrict__ rowout) {
+  __shared__ double sh[4][2];
+  const long b = blockIdx.x;
+  double vc = wave_sum(answer_sum(c, ignore, b)), vr = wave_sum(answer_sum(r, ignore, b));
+  if ((threadIdx.x & 63) == 0) {
+    sh[threadIdx.x >> 6][0] = vc;
+    sh[threadIdx.x >> 6][1] = vr;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  vc = sh[0][0] + sh[1][0] + sh[2][0] + sh[3][0];
+  vr = sh[0][1] + sh[1][1] + sh[2][1] + sh[3][1];
+  reward_c[b] = (float)(beta * vc);
+  reward_r[b] = (float)(beta * vr);
+  const float x = (float)(beta * (vc - vr));
+  const float q = expf(-fabsf(x)), l = log1pf(q);                    // -ln sig(|x|)
+  const float up = x >= 0.f ? l : l - x, down = x >= 0.f ? l + x : l;   // -ln sig(x), -ln sig(-x)
+  const float small = q / (1.f + q), large = 1.f / (1.f + q);           // sig(-|x|), sig(|x|)
+  const float sig = x >= 0.f ? large : small, gis = x >= 0.f ? small : large;
+  float loss = (1.f - smooth) * up;
+  if (smooth != 0.f) loss += smooth * down;
+  rowout[b] = make_float4(x != x ? x : loss, 0.f, 0.f, 0.f);
+  slope[b] = beta * (smooth * sig - (1.f - smooth) * gis);
+}
+// d logp of both answers: +- g * scale * slope on live tokens
+__global__ __launch_bounds__(256) void preference_bwd_kernel(const int64_t* __restrict__ labels_c, int Lc, float* __restrict__ dc,
+                                                             const int64_t* __restrict__ labels_r, int Lr, float* __restrict__ dr,
+                                                             int64_t ignore, long P, const float* __restrict__ slope, float scale,
+                                                             const float* __restrict__ g) {
+  const float w = *g * scale;
+  const long nc = P * Lc, n = nc + P * Lr;
+  for (long t = blockIdx.x * 256L + threadIdx.x; t < n; t += gridDim.x * 256L) {
+    if (t < nc)
+      dc[t] = labels_c[t] != ignore ? w * slope[t / Lc] : 0.f;
+    else
+      dr[t - nc] = labels_r[t - nc] != ignore ? -w * slope[(t - nc) / Lr] : 0.f;
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------------
+int check_rows(const char* who, const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp) {
+  PV_REQUIRE(logits && n0 > 0 && n1 > 0 && V > 0, "%s: null logits or an empty size", who);
+  PV_REQUIRE(dtype == PV_DTYPE_F32 || dtype == PV_DTYPE_BF16 || dtype == PV_DTYPE_F16, "%s: unknown dtype %d", who, dtype);
+  PV_REQUIRE(s0 >= 0 && s1 >= 0, "%s: negative stride", who);
+  PV_REQUIRE(inv_temp > 0.f && inv_temp < __builtin_inff(), "%s: the inverse temperature must be positive and finite", who);
+  PV_REQUIRE(((uintptr_t)logits & (dtype == PV_DTYPE_F32 ? 3 : 1)) == 0, "%s: logits not aligned to their elements", who);
+  if (V > kVocabMax || n0 * (long)n1 > 0x7fffffffL) {
+    pv_set_error("%s: %ld rows of %d words are beyond the limit (2^31 - 1 rows, 2^24 words)", who, n0 * (long)n1, V);
+    return PV_ERR_LIMIT;
+  }
+  return PV_OK;
+}
+Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, const int64_t* labels, int64_t ignore, float c) {
+  return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore};
+}
+
+template <int HEAD, bool ENT>
+int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
+  const dim3 grid((unsigned)a.T), block(256);
+  if (dtype == PV_DTYPE_F32)
+    rows_fwd_kernel<F32, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
+  else if (dtype == PV_DTYPE_BF16)
+    rows_fwd_kernel<BF16, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
+  else
+    rows_fwd_kernel<F16, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
+  PV_LAUNCH_CHECK("rows_fwd_kernel");
+  return PV_OK;
+}
+
+template <int HEAD>
+int launch_grad(int dtype, const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
+  const int item = 256 * 4 * (dtype == PV_DTYPE_F32 ? 4 : 8);
+  const int blocks = cdiv(a.V, item);
+  const long items = a.T * blocks;
+  const dim3 grid((unsigned)(items < 4096 ? items : 4096)), block(256);
+  if (dtype == PV_DTYPE_F32)
+    rows_grad_kernel<F32, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
+  else if (dtype == PV_DTYPE_BF16)
+    rows_grad_kernel<BF16, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
+  else
+    rows_grad_kernel<F16, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
+  PV_LAUNCH_CHECK("rows_grad_kernel");
+  return PV_OK;
+}
+
+int launch_count(const int64_t* labels, int64_t ignore, long T, float* part, float* out, hipStream_t st) {
+  const int g = sum_groups(T);
+  count_live_kernel<<<dim3(g), dim3(1024), 0, st>>>(labels, ignore, T, part, out);
+  PV_LAUNCH_CHECK("count_live_kernel");
+  if (g > 1) {
+    add_counts_kernel<<<dim3(1), dim3(256), 0, st>>>(part, g, out);
+    PV_LAUNCH_CHECK("add_counts_kernel");
+  }
+  return PV_OK;
+}
+int launch_sum(const float4* rows, const int64_t* labels, int64_t ignore, long T, Sum5* part, const Result& r, hipStream_t st) {
+  const int g = sum_groups(T);
+  sum_rows_kernel<<<dim3(g), dim3(1024), 0, st>>>(rows, labels, ignore, T, part, r);
+  PV_LAUNCH_CHECK("sum_rows_kernel");
+  if (g > 1) {
+    sum_parts_kernel<<<dim3(1), dim3(256), 0, st>>>(part, g, r);
+    PV_LAUNCH_CHECK("sum_parts_kernel");
+  }
+  return PV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pv_vocab_rows_ws_bytes(long rows) {
+  return rows < 0 ? 0 : (size_t)rows * sizeof(float4) + kSumGroups * sizeof(Sum5) + sizeof(float);
+}
+
+int pv_token_logp_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                      int64_t ignore, float inv_temp, float* logp, float* entropy, float* save, void* stream) {
+  const int rc = check_rows("pv_token_logp_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(tokens && logp, "pv_token_logp_fwd: null argument");
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  const FwdOut o = {logp, entropy, nullptr, (float4*)save};
+  if (entropy) return launch_fwd<HEAD_TOKEN, true>(dtype, a, Policy{}, Distill{}, Scale{}, o, (hipStream_t)stream);
+  return launch_fwd<HEAD_TOKEN, false>(dtype, a, Policy{}, Distill{}, Scale{}, o, (hipStream_t)stream);
+}
+
+int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                      int64_t ignore, float inv_temp, const float* save, const float* dlogp, const float* dentropy,
+                      void* dlogits, void* stream) {
+  const int rc = check_rows("pv_token_logp_bwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(tokens && save && dlogits && (dlogp || dentropy), "pv_token_logp_bwd: null argument");
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, dlogp, dentropy, nullptr, dlogits},
+                                 (hipStream_t)stream);
+}
+
+int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                       int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
+                       int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
+                       float* loss, float* stats, float* save, void* ws, void* stream) {
+  const int rc = check_rows("pv_policy_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(tokens && old_logp && adv && loss && stats && ws, "pv_policy_rows_fwd: null argument");
+  PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_rows_fwd: the clip range is empty");
+  hipStream_t st = (hipStream_t)stream;
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  float4* rowout = (float4*)ws;
+  Sum5* part = (Sum5*)(rowout + a.T);
+  Scale sc = {weight, nullptr};
+  if (word && save) {
+    float* count = (float*)(part + kSumGroups);
+    const int r = launch_count(tokens, ignore, a.T, (float*)part, count, st);
+    if (r != PV_OK) return r;
+    sc.count = count;
+  }
+  const Policy hp = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, ent_coef};
+  const int r = launch_fwd<HEAD_POLICY, true>(dtype, a, hp, Distill{}, sc, FwdOut{nullptr, nullptr, rowout, (float4*)save}, st);
+  if (r != PV_OK) return r;
+  return launch_sum(rowout, tokens, ignore, a.T, part, Result{kl_coef, ent_coef, weight, word, loss, stats, nullptr}, st);
+}
+
+int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
+                       int64_t ignore, float inv_temp, const float* save, const float* g, void* dlogits, void* stream) {
+  const int rc = check_rows("pv_policy_rows_bwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(tokens && save && g && dlogits, "pv_policy_rows_bwd: null argument");
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  return launch_grad<HEAD_POLICY>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, g, dlogits},
+                                  (hipStream_t)stream);
+}
+
+int pv_distill_max_entries(void) { return kTeacherMax; }
+
+int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
+                        int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
+                        float weight, int word, float* loss, float* save, float* psum, void* ws, void* stream) {
+  const int rc = check_rows("pv_distill_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(t_ids && t_logits && loss && psum && ws, "pv_distill_rows_fwd: null argument");
+  PV_REQUIRE(t_dtype == PV_DTYPE_F32 || t_dtype == PV_DTYPE_BF16 || t_dtype == PV_DTYPE_F16,
+             "pv_distill_rows_fwd: unknown teacher dtype %d", t_dtype);
+  PV_REQUIRE(K > 0, "pv_distill_rows_fwd: no teacher entries");
+  if (K > kTeacherMax) {
+    pv_set_error("pv_distill_rows_fwd: %d teacher entries are beyond the limit of %d", K, kTeacherMax);
+    return PV_ERR_LIMIT;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, labels, ignore, inv_temp);
+  float4* rowout = (float4*)ws;
+  Sum5* part = (Sum5*)(rowout + a.T);
+  Scale sc = {weight, nullptr};
+  if (word && !labels) sc.weight = weight / (float)a.T;
+  if (word && labels && save) {
+    float* count = (float*)(part + kSumGroups);
+    const int r = launch_count(labels, ignore, a.T, (float*)part, count, st);
+    if (r != PV_OK) return r;
+    sc.count = count;
+  }
+  const Distill hd = {t_ids, t_logits, K, t_dtype, psum};
+  const int r = launch_fwd<HEAD_DISTILL, false>(dtype, a, Policy{}, hd, sc, FwdOut{nullptr, nullptr, rowout, (float4*)save}, st);
+  if (r != PV_OK) return r;
+  return launch_sum(rowout, labels, ignore, a.T, part, Result{0.f, 0.f, weight, word, loss, nullptr, nullptr}, st);
+}
+
+int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp,
+                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, void* dlogits,
+                        void* stream) {
+  const int rc = check_rows("pv_distill_rows_bwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(t_ids && save && psum && g && dlogits && K > 0 && K <= kTeacherMax, "pv_distill_rows_bwd: bad argument");
+  const Rows a = make_rows(logits, n0, n1, s0, s1, V, nullptr, 0, inv_temp);
+  return launch_grad<HEAD_DISTILL>(dtype, a, Distill{t_ids, nullptr, K, 0, (float*)psum},
+                                   Grad{(const float4*)save, nullptr, nullptr, g, dlogits}, (hipStream_t)stream);
+}
+
+int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,
+                         const float* ref_logp, const float* adv, int adv_per_token, float clip_lo, float clip_hi,
+                         float kl_coef, float weight, int word, float* loss, float* stats, float* dlogp, void* ws, void* stream) {
+  PV_REQUIRE(logp && tokens && old_logp && adv && loss && stats && ws && n0 > 0 && n1 > 0, "pv_policy_tokens_fwd: bad argument");
+  PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_tokens_fwd: the clip range is empty");
+  hipStream_t st = (hipStream_t)stream;
+  const long T = n0 * (long)n1;
+  const Policy h = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, 0.f};
+  const Result r = {kl_coef, 0.f, weight, word, loss, stats, dlogp ? dlogp + T : nullptr};
+  const long want = (T + 1023) / 1024;
+  const int g = (int)(want > kSumGroups ? kSumGroups : want);
+  policy_tokens_kernel<<<dim3(g), dim3(256), 0, st>>>(logp, tokens, ignore, T, n1, h, dlogp, (Sum5*)ws, r);
+  PV_LAUNCH_CHECK("policy_tokens_kernel");
+  if (g > 1) {
+    sum_parts_kernel<<<dim3(1), dim3(256), 0, st>>>((const Sum5*)ws, g, r);
+    PV_LAUNCH_CHECK("sum_parts_kernel");
+  }
+  return PV_OK;
+}
+
+int pv_policy_tokens_bwd(const float* dlogp, const float* g, long n, float* d, void* stream) {
+  PV_REQUIRE(dlogp && g && d && n > 0, "pv_policy_tokens_bwd: bad argument");
+  const long want = (n + 255) / 256;
+  policy_tokens_bwd_kernel<<<dim3((unsigned)(want > 2048 ? 2048 : want)), dim3(256), 0, (hipStream_t)stream>>>(
+      dlogp, dlogp + n, g, n, d);
+  PV_LAUNCH_CHECK("policy_tokens_bwd_kernel");
+  return PV_OK;
+}
+
+int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* labels_c, int Lc, const float* logp_r,
+                      const float* ref_r, const int64_t* labels_r, int Lr, long pairs, int64_t ignore, float beta,
+                      float smoothing, float weight, float* loss, float* rewards, float* slope, void* ws, void* stream) {
+  PV_REQUIRE(loss && rewards && slope && ws && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_fwd: bad argument");
+  PV_REQUIRE((Lc == 0 || (logp_c && labels_c)) && (Lr == 0 || (logp_r && labels_r)), "pv_preference_fwd: null argument");
+  if (pairs > 0x7fffffffL) {
+    pv_set_error("pv_preference_fwd: %ld pairs are beyond the limit of 2^31 - 1", pairs);
+    return PV_ERR_LIMIT;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  float4* rowout = (float4*)ws;
+  preference_kernel<<<dim3((unsigned)pairs), dim3(256), 0, st>>>(Answers{logp_c, ref_c, labels_c, Lc},
+                                                                 Answers{logp_r, ref_r, labels_r, Lr}, ignore, beta, smoothing,
+                                                                 rewards, rewards + pairs, slope, rowout);
+  PV_LAUNCH_CHECK("preference_kernel");
+  return launch_sum(rowout, nullptr, 0, pairs, (Sum5*)(rowout + pairs), Result{0.f, 0.f, weight, 0, loss, nullptr, nullptr}, st);
+}
+
+int pv_preference_bwd(const int64_t* labels_c, int Lc, const int64_t* labels_r, int Lr, long pairs, int64_t ignore,
+                      const float* slope, float weight, const float* g, float* dlogp_c, float* dlogp_r, void* stream) {
+  PV_REQUIRE(slope && g && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_bwd: bad argument");
+  PV_REQUIRE((Lc == 0 || (labels_c && dlogp_c)) && (Lr == 0 || (labels_r && dlogp_r)), "pv_preference_bwd: null argument");
+  const long n = pairs * ((long)Lc + Lr), want = (n + 255) / 256;
+  if (n == 0) return PV_OK;
+  preference_bwd_kernel<<<dim3((unsigned)(want > 2048 ? 2048 : want)), dim3(256), 0, (hipStream_t)stream>>>(
+      labels_c, Lc, dlogp_c, labels_r, Lr, dlogp_r, ignore, pairs, slope, weight, g);
+  PV_LAUNCH_CHECK("preference_bwd_kernel");
+  return PV_OK;
+}
+
+}  // extern "C"

@@ -75,6 +75,7 @@ class DeferredLogProbs(object):
         self.hid_bf16, self.layout, self.drop = hid_bf16, layout, drop
         self._dense = None
         self._nll_cache = {}
+        self._nll_labels = []
 
     # -- what the criterions use -------------------------------------------------------------------------
     def token_nll(self, labels, ignore_index, sums_only=False):
@@ -85,6 +86,7 @@ class DeferredLogProbs(object):
         hit = self._nll_cache.get(key)
         if hit is not None:
             return hit + (False,)
+        self._nll_labels.append(labels)          # the cache goes by address: no other labels may come to lie there
         B, L, H = self.hid.shape
         if self.hid_bf16 is not None or (self.drop is not None and self.layout is not None):
             Lh, Bh, Bpad = self.layout
@@ -135,6 +137,14 @@ class DeferredLogProbs(object):
         if hit is None:
             hit = self._nll_cache[key] = ops.NllHead.apply(self._sums(labels, ignore_index), self.hid.shape[0])
         return hit
+
+    def token_logp(self, labels, ignore_index):
+        """Log-probability of `labels` [B, L] (0 where label == ignore_index) without the logits, differentiable."""
+        B, L, _ = self.hid.shape
+        nll = self.token_nll(labels, ignore_index)[0]
+        if self.hid_bf16 is not None or (self.drop is not None and self.layout is not None):     # rows t * Bpad + b
+            return -nll.view(L, self.layout[2])[:, :B].t()
+        return -nll.view(B, L)
 
     # -- dense fallback: behaves like the reference's tensor ---------------------------------------------------
     def materialize(self):

@@ -2674,3 +2674,378 @@ def cons_loss_sum(pairs):
 def cons_loss(v1, v2):
     """DLS_Auto.cons_loss (dialog_models.py:3266-3272) with batch_arrange = arange(B)."""
     return InfoNCE.apply(ScaledMatmulNT.apply(L2NormRows.apply(v1), L2NormRows.apply(v2), 1.1))
+
+
+# ------------------------------------------------------------------------------------------------------------
+# losses over rows of a vocabulary softmax in memory: token log-probabilities, distillation from a teacher's top logits,
+# clipped policy loss, preference loss
+# ------------------------------------------------------------------------------------------------------------
+
+_ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NO_INDEX = -(1 << 63)           # an ignore index that no label has
+
+
+def _launch(dev, name, *args):
+    """One C call on `dev`'s current stream, whatever the current device is."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _same_device(*ts):
+    _need_cuda(*ts)
+    dev = ts[0].device
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError("tensors on different devices: %s and %s" % (dev, t.device))
+    return dev
+
+
+def _constant(name, t, shape):
+    """A tensor that carries no gradient here, as contiguous fp32 of the given shape."""
+    if t is None:
+        return None
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s is a constant of this loss: detach it" % name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if not t.dtype.is_floating_point:
+        raise ValueError("%s must be floating point (got %s)" % (name, t.dtype))
+    return t.detach().to(torch.float32).contiguous()
+
+
+def _index(name, t, shape):
+    if t.dtype not in (torch.int64, torch.int32):
+        raise ValueError("%s must be int64 or int32 (got %s)" % (name, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    return t.to(torch.int64).contiguous()
+
+
+def _check_rows(logits):
+    if logits.dtype not in _ROW_DTYPES:
+        raise ValueError("logits must be float32, bfloat16 or float16 (got %s)" % logits.dtype)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits need a last dimension of at least one word (got shape %s)" % (tuple(logits.shape),))
+
+
+def _check_temp(x):
+    if not 0.0 < x < float("inf"):
+        raise ValueError("the temperature must be positive and finite (got %r)" % (x,))
+
+
+def _row_args(x):
+    """The leading C arguments (pointer, dtype, n0, n1, s0, s1, V) of rows whose words are contiguous; up to three
+    dimensions keep their strides."""
+    V = x.shape[-1]
+    if x.dim() == 1:
+        n0, n1, s0, s1 = 1, 1, 0, 0
+    elif x.dim() == 2:
+        n0, n1, s0, s1 = 1, x.shape[0], 0, x.stride(0)
+    else:
+        n0, n1, s0, s1 = x.shape[0], x.shape[1], x.stride(0), x.stride(1)
+    return _p(x), _ROW_DTYPES[x.dtype], n0, n1, s0, s1, V
+
+
+def _plain_rows(x):
+    """`x` itself where the kernels can read it in place, else a contiguous copy of its rows."""
+    if x.dim() > 3:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _avg(avg_type, weight, sequences):
+    """(weight, word) of the C calls: 'seq' = sum / sequences, 'word' = mean over live tokens, None = sum."""
+    if avg_type == "seq":
+        return float(weight) / max(sequences, 1), 0
+    if avg_type == "word":
+        return float(weight), 1
+    if avg_type is None:
+        return float(weight), 0
+    raise ValueError("Unknown avg type")
+
+
+class TokenLogProbs(torch.autograd.Function):
+    """log_softmax(logits * inv_temp)[token] and the entropy of a row; the log-softmax itself is never written."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, ignore, inv_temp, entropy, want_grad):
+        x = _plain_rows(logits)
+        dev, shape = x.device, logits.shape[:-1]
+        logp = torch.empty(shape, dtype=torch.float32, device=dev)
+        ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
+        save = torch.empty((tokens.numel(), 4), dtype=torch.float32, device=dev) if want_grad else None
+        _launch(dev, "pv_token_logp_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(logp), _p(ent), _p(save))
+        if want_grad:
+            ctx.save_for_backward(x, tokens, save)
+        ctx.meta = (ignore, inv_temp, logits.shape)
+        ctx.set_materialize_grads(False)
+        return (logp, ent) if entropy else logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dent=None):
+        if dlogp is None and dent is None:
+            return (None,) * 6
+        x, tokens, save = ctx.saved_tensors
+        ignore, inv_temp, shape = ctx.meta
+        dlogp = None if dlogp is None else dlogp.to(torch.float32).contiguous()
+        dent = None if dent is None else dent.to(torch.float32).contiguous()
+        d = torch.empty(shape, dtype=x.dtype, device=x.device)
+        _launch(x.device, "pv_token_logp_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(save), _p(dlogp), _p(dent), _p(d))
+        return d, None, None, None, None, None
+
+
+def token_logprobs(logits, tokens, ignore_index=None, inv_temp=1.0, entropy=False):
+    """Log-probability of `tokens` [...] under softmax(logits [..., V] * inv_temp), fp32, and with `entropy` the entropy of
+    every row as well -> logp or (logp, entropy), both differentiable in `logits` (float32 / bfloat16 / float16, any strides;
+    log-probabilities serve as logits).  Rows whose token is `ignore_index` are not read: 0, with a zero gradient.  Any other
+    token outside [0, V) makes its row NaN."""
+    _check_rows(logits)
+    tokens = _index("tokens", tokens, logits.shape[:-1])
+    _check_temp(inv_temp)
+    _same_device(logits, tokens)
+    if tokens.numel() == 0:
+        z = logits.to(torch.float32).sum(-1)
+        return (z, z) if entropy else z
+    want = logits.requires_grad and torch.is_grad_enabled()
+    return TokenLogProbs.apply(logits, tokens, _NO_INDEX if ignore_index is None else int(ignore_index), float(inv_temp),
+                               bool(entropy), want)
+
+
+class DistillTopK(torch.autograd.Function):
+    """KL(teacher's softmax over its top entries || softmax(logits)) at a temperature, summed over live rows."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, t_logits, labels, ignore, inv_temp, weight, word, want_grad):
+        x = _plain_rows(logits)
+        dev, K = x.device, ids.shape[-1]
+        T = ids.numel() // K
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
+        psum = torch.empty((T, K), dtype=torch.float32, device=dev)
+        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
+        _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, _p(ids), _p(t_logits),
+                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), _p(save), _p(psum), _p(ws))
+        if want_grad:
+            ctx.save_for_backward(x, ids, save, psum)
+        ctx.meta = (inv_temp, K, logits.shape)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, ids, save, psum = ctx.saved_tensors
+        inv_temp, K, shape = ctx.meta
+        d = torch.empty(shape, dtype=x.dtype, device=x.device)
+        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(save), _p(psum), _p(g.contiguous()), _p(d))
+        return (d,) + (None,) * 8
+
+
+def distill_topk(logits, teacher_ids, teacher_logits, labels=None, ignore_index=None, temperature=1.0, weight=1.0,
+                 avg_type="seq"):
+    """Distillation of `logits` [..., V] from a teacher's top logits: teacher_ids (int) / teacher_logits [..., K], K <= 256.
+    With p the softmax of a row's teacher logits and q that of its logits, both at `temperature`:
+    weight * temperature^2 * sum_j p_j (log p_j - log q[id_j]), summed over rows and averaged by `avg_type` ('seq': sequences,
+    the first dimension; 'word': live rows; None: sum) -> fp32 scalar, differentiable in `logits`.
+
+    Entries of -inf do not count (lists of different lengths are padded with them); a word that is listed twice counts with
+    both entries.  Rows whose label is `ignore_index` are dead; without labels every row is live.  An entry that counts and
+    names no word makes the loss NaN.  A coefficient belongs into `weight`: an upstream gradient other than 1 costs another
+    pass over the rows."""
+    _check_rows(logits)
+    lead = tuple(logits.shape[:-1])
+    K_max = _lib.load().pv_distill_max_entries()
+    if teacher_logits.dim() != logits.dim() or tuple(teacher_logits.shape[:-1]) != lead or teacher_logits.shape[-1] < 1:
+        raise ValueError("teacher_logits has shape %s, expected %s" % (tuple(teacher_logits.shape), lead + ("K",)))
+    if teacher_logits.shape[-1] > K_max:
+        raise ValueError("%d teacher entries a row, at most %d are taken" % (teacher_logits.shape[-1], K_max))
+    if teacher_logits.dtype not in _ROW_DTYPES:
+        raise ValueError("teacher_logits must be float32, bfloat16 or float16 (got %s)" % teacher_logits.dtype)
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("teacher_logits is a constant of this loss: detach it")
+    teacher_ids = _index("teacher_ids", teacher_ids, teacher_logits.shape)
+    if labels is not None:
+        labels = _index("labels", labels, lead)
+    _check_temp(temperature)
+    w, word = _avg(avg_type, weight, logits.shape[0] if logits.dim() > 1 else 1)
+    _same_device(logits, teacher_ids, teacher_logits, labels)
+    if teacher_ids.numel() == 0:
+        return logits.to(torch.float32).sum() * 0.0
+    want = logits.requires_grad and torch.is_grad_enabled()
+    return DistillTopK.apply(logits, teacher_ids, teacher_logits.detach().contiguous(), labels,
+                             _NO_INDEX if ignore_index is None else int(ignore_index), 1.0 / float(temperature), w, word, want)
+
+
+class VocabPolicyLoss(torch.autograd.Function):
+    """The clipped policy loss of sampled tokens from the logits of their rows."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, old, ref, adv, ignore, inv_temp, lo, hi, kl, ent, weight, word, want_grad):
+        x = _plain_rows(logits)
+        dev, T = x.device, tokens.numel()
+        loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
+        save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
+        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
+        _launch(dev, "pv_policy_rows_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(old), _p(ref), _p(adv),
+                int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), _p(save), _p(ws))
+        if want_grad:
+            ctx.save_for_backward(x, tokens, save)
+        ctx.meta = (ignore, inv_temp, logits.shape)
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _dstats):
+        x, tokens, save = ctx.saved_tensors
+        ignore, inv_temp, shape = ctx.meta
+        d = torch.empty(shape, dtype=x.dtype, device=x.device)
+        _launch(x.device, "pv_policy_rows_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(save), _p(g.contiguous()), _p(d))
+        return (d,) + (None,) * 13
+
+
+class PolicyLoss(torch.autograd.Function):
+    """The clipped policy loss from the tokens' log-probabilities."""
+
+    @staticmethod
+    def forward(ctx, logp, tokens, old, ref, adv, ignore, lo, hi, kl, weight, word, want_grad):
+        x = logp.contiguous()
+        dev, T = x.device, tokens.numel()
+        n1 = x.shape[1] if x.dim() == 2 else T
+        loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
+        dlp = torch.empty(T + 1, dtype=torch.float32, device=dev) if want_grad else None
+        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(0), dtype=torch.uint8, device=dev)
+        _launch(dev, "pv_policy_tokens_fwd", _p(x), _p(tokens), ignore, T // n1, n1, _p(old), _p(ref), _p(adv),
+                int(adv.numel() == T), lo, hi, kl, weight, word, _p(loss), _p(stats), _p(dlp), _p(ws))
+        if want_grad:
+            ctx.save_for_backward(dlp)
+        ctx.shape = logp.shape
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _dstats):
+        dlp, = ctx.saved_tensors
+        d = torch.empty(ctx.shape, dtype=torch.float32, device=dlp.device)
+        _launch(dlp.device, "pv_policy_tokens_bwd", _p(dlp), _p(g.contiguous()), d.numel(), _p(d))
+        return (d,) + (None,) * 11
+
+
+def _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef):
+    old, ref = _constant("old_logp", old_logp, shape), _constant("ref_logp", ref_logp, shape)
+    per_token = tuple(advantages.shape) == tuple(shape)
+    adv = _constant("advantages", advantages, shape if per_token or len(shape) < 2 else shape[:1])
+    clip_high = clip if clip_high is None else clip_high
+    if not (clip >= 0 and clip_high >= 0):
+        raise ValueError("the clip range must not be negative (got %r, %r)" % (clip, clip_high))
+    if kl_coef != 0 and ref is None:
+        raise ValueError("kl_coef needs ref_logp")
+    return old, ref, adv, 1.0 - float(clip), 1.0 + float(clip_high), float(kl_coef)
+
+
+def vocab_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, ignore_index=None, inv_temp=1.0, clip=0.2,
+                      clip_high=None, kl_coef=0.0, ent_coef=0.0, weight=1.0, avg_type="word"):
+    """Clipped policy loss of sampled `tokens` [B, L] (or [T]) from the logits [B, L, V] of their rows.  With log-probabilities
+    logp of the tokens, r = exp(logp - old_logp), d = ref_logp - logp and the rows' entropy H, a live token adds
+    -min(r A, clip(r, 1 - clip, 1 + clip_high) A) + kl_coef (exp(d) - 1 - d) - ent_coef H; averaged by `avg_type` ('word': live
+    tokens, 'seq': sequences, None: sum) and multiplied by `weight`.  advantages: one a token, or one a sequence [B].
+    -> (loss, stats): an fp32 scalar differentiable in `logits`, and the means over live tokens of the policy term, of the KL
+    term, of "the clip decides" and of H.  old_logp, ref_logp and advantages are constants.  Dead rows (`ignore_index`) are
+    not read.  A coefficient belongs into `weight`: an upstream gradient other than 1 costs another pass over the rows."""
+    _check_rows(logits)
+    shape = tuple(logits.shape[:-1])
+    if not 1 <= len(shape) <= 2:
+        raise ValueError("logits must be [B, L, V] or [T, V] (got shape %s)" % (tuple(logits.shape),))
+    tokens = _index("tokens", tokens, shape)
+    old, ref, adv, lo, hi, kl = _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef)
+    _check_temp(inv_temp)
+    w, word = _avg(avg_type, weight, shape[0])
+    _same_device(logits, tokens, old_logp, advantages, ref_logp)
+    if tokens.numel() == 0:
+        return logits.to(torch.float32).sum() * 0.0, torch.zeros(4, dtype=torch.float32, device=logits.device)
+    want = logits.requires_grad and torch.is_grad_enabled()
+    return VocabPolicyLoss.apply(logits, tokens, old, ref, adv, _NO_INDEX if ignore_index is None else int(ignore_index),
+                                 float(inv_temp), lo, hi, kl, float(ent_coef), w, word, want)
+
+
+def policy_loss(logp, tokens, old_logp, advantages, ref_logp=None, ignore_index=None, clip=0.2, clip_high=None, kl_coef=0.0,
+                weight=1.0, avg_type="word"):
+    """vocab_policy_loss from the tokens' log-probabilities `logp` [B, L] (or [T]), as token_logprobs or the fused vocabulary
+    projection gives them; no entropy term.  -> (loss, stats), the last of the stats 0."""
+    shape = tuple(logp.shape)
+    if not 1 <= len(shape) <= 2 or logp.dtype != torch.float32:
+        raise ValueError("logp must be float32 [B, L] or [T] (got %s %s)" % (logp.dtype, shape))
+    tokens = _index("tokens", tokens, shape)
+    old, ref, adv, lo, hi, kl = _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef)
+    w, word = _avg(avg_type, weight, shape[0])
+    _same_device(logp, tokens, old_logp, advantages, ref_logp)
+    if tokens.numel() == 0:
+        return logp.sum() * 0.0, torch.zeros(4, dtype=torch.float32, device=logp.device)
+    want = logp.requires_grad and torch.is_grad_enabled()
+    return PolicyLoss.apply(logp, tokens, old, ref, adv, _NO_INDEX if ignore_index is None else int(ignore_index), lo, hi, kl, w,
+                            word, want)
+
+
+class PreferenceLoss(torch.autograd.Function):
+    """The preference loss of pairs of answers from their tokens' log-probabilities."""
+
+    @staticmethod
+    def forward(ctx, logp_c, logp_r, labels_c, labels_r, ref_c, ref_r, ignore, beta, smoothing, weight):
+        xc, xr = logp_c.contiguous(), logp_r.contiguous()
+        dev, P = xc.device, xc.shape[0]
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
+        slope = torch.empty(P, dtype=torch.float32, device=dev)
+        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(P), dtype=torch.uint8, device=dev)
+        _launch(dev, "pv_preference_fwd", _p(xc), _p(ref_c), _p(labels_c), xc.shape[1], _p(xr), _p(ref_r), _p(labels_r),
+                xr.shape[1], P, ignore, beta, smoothing, weight, _p(loss), _p(rewards), _p(slope), _p(ws))
+        ctx.save_for_backward(labels_c, labels_r, slope)
+        ctx.meta = (ignore, weight)
+        rc, rr = rewards[0], rewards[1]
+        ctx.mark_non_differentiable(rc, rr)
+        return loss, rc, rr
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _drc, _drr):
+        labels_c, labels_r, slope = ctx.saved_tensors
+        ignore, weight = ctx.meta
+        dc = torch.empty(labels_c.shape, dtype=torch.float32, device=slope.device)
+        dr = torch.empty(labels_r.shape, dtype=torch.float32, device=slope.device)
+        _launch(slope.device, "pv_preference_bwd", _p(labels_c), labels_c.shape[1], _p(labels_r), labels_r.shape[1],
+                slope.numel(), ignore, _p(slope), weight, _p(g.contiguous()), _p(dc), _p(dr))
+        return (dc, dr) + (None,) * 8
+
+
+def preference_loss(chosen_logp, chosen_labels, rejected_logp, rejected_labels, ref_chosen=None, ref_rejected=None,
+                    ignore_index=None, beta=0.1, label_smoothing=0.0, weight=1.0, avg_type="seq"):
+    """Preference loss over P pairs of answers from their tokens' log-probabilities [P, Lc] / [P, Lr] (fp32).  With the rewards
+    beta * sum over live tokens of (logp - ref) and x = chosen - rejected reward, a pair adds
+    -(1 - label_smoothing) ln sig(x) - label_smoothing ln sig(-x); averaged over pairs ('seq') or summed (None), times `weight`.
+    -> (loss, chosen rewards [P], rejected rewards [P]); the loss is differentiable in both log-probabilities.  The reference
+    model's log-probabilities are constants (both None: no reference model).  Labels of `ignore_index` are not read."""
+    for name, t in (("chosen_logp", chosen_logp), ("rejected_logp", rejected_logp)):
+        if t.dim() != 2 or t.dtype != torch.float32:
+            raise ValueError("%s must be float32 [P, L] (got %s %s)" % (name, t.dtype, tuple(t.shape)))
+    if chosen_logp.shape[0] != rejected_logp.shape[0]:
+        raise ValueError("%d chosen and %d rejected answers" % (chosen_logp.shape[0], rejected_logp.shape[0]))
+    if (ref_chosen is None) != (ref_rejected is None):
+        raise ValueError("a reference model's log-probabilities are needed for both answers, or for neither")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("label_smoothing must lie in [0, 1] (got %r)" % (label_smoothing,))
+    if avg_type not in ("seq", None):
+        raise ValueError("Unknown avg type")
+    lc = _index("chosen_labels", chosen_labels, chosen_logp.shape)
+    lr = _index("rejected_labels", rejected_labels, rejected_logp.shape)
+    rc, rr = _constant("ref_chosen", ref_chosen, chosen_logp.shape), _constant("ref_rejected", ref_rejected, rejected_logp.shape)
+    _same_device(chosen_logp, chosen_labels, rejected_logp, rejected_labels, ref_chosen, ref_rejected)
+    P = chosen_logp.shape[0]
+    if P == 0:
+        z = torch.zeros(0, dtype=torch.float32, device=chosen_logp.device)
+        return (chosen_logp.sum() + rejected_logp.sum()) * 0.0, z, z.clone()
+    return PreferenceLoss.apply(chosen_logp, rejected_logp, lc, lr, rc, rr, _NO_INDEX if ignore_index is None else int(ignore_index),
+                                float(beta), float(label_smoothing), _avg(avg_type, weight, P)[0])

@@ -1,0 +1,93 @@
+"""Losses over rows of a vocabulary softmax in memory (ops.token_logprobs, distill_topk, vocab_policy_loss, policy_loss,
+preference_loss and their criterions): what they refuse, without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from pevae_amd import _lib, criterions, ops
+
+
+def rows(B=2, L=3, V=5, dtype=torch.float32):
+    return torch.zeros(B, L, V, dtype=dtype)
+
+
+def ids(*shape):
+    return torch.ones(*shape, dtype=torch.int64)
+
+
+def f(*shape):
+    return torch.zeros(*shape)
+
+
+def test_valid_arguments_on_the_cpu_raise_for_the_device():
+    for call in (lambda: ops.token_logprobs(rows(), ids(2, 3)),
+                 lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2), ids(2, 3), 0),
+                 lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(2)),
+                 lambda: ops.policy_loss(f(2, 3), ids(2, 3), f(2, 3), f(2, 3)),
+                 lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 4), ids(2, 4))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.token_logprobs(rows(dtype=torch.float64), ids(2, 3)),                       # type
+    lambda: ops.token_logprobs(rows(V=0), ids(2, 3)),                                       # no words
+    lambda: ops.token_logprobs(rows(), ids(3, 2)),                                          # shape
+    lambda: ops.token_logprobs(rows(), f(2, 3)),                                            # tokens are no integers
+    lambda: ops.token_logprobs(rows(), ids(2, 3), inv_temp=0.0),
+    lambda: ops.token_logprobs(rows(), ids(2, 3), inv_temp=float("nan")),
+    lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 3)),                             # ids and logits differ
+    lambda: ops.distill_topk(rows(), ids(2, 3, 0), f(2, 3, 0)),                             # no entries
+    lambda: ops.distill_topk(rows(), ids(2, 3, 257), f(2, 3, 257)),                         # too many
+    lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2).requires_grad_()),            # no gradient for the teacher
+    lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2), ids(2, 4)),
+    lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2), temperature=0.0),
+    lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2), avg_type="real_word"),
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(3)),                        # advantages
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 2), f(2)),                        # old_logp
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(2), kl_coef=0.1),           # no reference model
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(2), clip=-0.1),
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3).requires_grad_(), f(2)),
+    lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), ids(2)),                      # integer advantages
+    lambda: ops.vocab_policy_loss(torch.zeros(1, 2, 3, 5), ids(1, 2, 3), f(1, 2, 3), f(1)),
+    lambda: ops.policy_loss(f(2, 3).double(), ids(2, 3), f(2, 3), f(2)),
+    lambda: ops.policy_loss(f(2, 3), ids(2, 3), f(2, 3), f(2), avg_type="mean"),
+    lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(3, 3), ids(3, 3)),                    # not pairs
+    lambda: ops.preference_loss(f(6), ids(6), f(6), ids(6)),
+    lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), ref_chosen=f(2, 3)),
+    lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), label_smoothing=1.5),
+    lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), avg_type="word"),
+])
+def test_bad_arguments_raise_value_errors(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_criterions_refuse_unknown_averages():
+    for cls in (criterions.TopKDistill, criterions.ClippedPolicyLoss, criterions.PreferenceLoss):
+        with pytest.raises(NotImplementedError):
+            cls(0, None, avg_type="real_word")
+
+
+def test_entry_points_refuse_on_the_host():
+    """Nothing is launched for bad sizes, types, null pointers, or sizes beyond the limits."""
+    lib = _lib.load()
+    p = C.c_void_p(64)
+
+    def logp(logits=p, dtype=0, n0=1, n1=4, s0=0, s1=5, V=5, tokens=p, temp=1.0, out=p):
+        return lib.pv_token_logp_fwd(logits, dtype, n0, n1, s0, s1, V, tokens, 0, temp, out, None, None, None)
+
+    for bad in (dict(logits=None), dict(dtype=3), dict(n0=0), dict(n1=0), dict(V=0), dict(tokens=None), dict(out=None), dict(temp=0.0),
+                dict(temp=float("inf")), dict(s1=-5), dict(logits=C.c_void_p(66)), dict(logits=C.c_void_p(65), dtype=1)):
+        assert logp(**bad) == -1, bad
+        assert b"pv_token_logp_fwd" in lib.pv_last_error()
+    assert logp(n0=1 << 16, n1=1 << 15) == -3
+    assert logp(V=(1 << 24) + 1) == -3
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, p, None) == -3
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, p, None) == -1
+    assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, p, None) == -1
+    assert lib.pv_policy_tokens_fwd(p, p, 0, 0, 4, p, None, p, 0, 0.8, 1.2, 0.0, 1.0, 0, p, p, p, p, None) == -1
+    assert lib.pv_preference_fwd(None, None, None, 3, p, None, p, 3, 2, 0, 0.1, 0.0, 1.0, p, p, p, p, None) == -1
+    assert lib.pv_distill_max_entries() == 256
+    assert lib.pv_vocab_rows_ws_bytes(10) >= 160
