@@ -537,6 +537,10 @@ int pv_dropout_pack_bf16(const float* src, int n0, int n1, int n1p, int C, long 
 #define PV_DTYPE_BF16 1
 #define PV_DTYPE_F16 2
 size_t pv_vocab_rows_ws_bytes(long rows);
+/* Whether rows of V words fit the one-pass form of the policy and distillation calls: forward with dlogits != NULL (and
+ * save) writes the gradient for an upstream gradient of 1 as well, and backward with ready != 0 and the same dlogits leaves it
+ * where *g is 1 and computes it afresh where it is not. */
+int pv_vocab_rows_one_pass(int dtype, int V);
 /* logp[t] = log_softmax(logits * inv_temp)[t][tokens[t]]; entropy[t] (NULL: not wanted) of the same distribution.  Backward
  * for upstream gradients dlogp / dentropy [rows] (either may be NULL). */
 int pv_token_logp_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
@@ -552,9 +556,9 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
 int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                        int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
                        int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
-                       float* loss, float* stats, float* save, void* ws, void* stream);
+                       float* loss, float* stats, float* save, void* dlogits, void* ws, void* stream);
 int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
-                       int64_t ignore, float inv_temp, const float* save, const float* g, void* dlogits, void* stream);
+                       int64_t ignore, float inv_temp, const float* save, const float* g, int ready, void* dlogits, void* stream);
 /* Distillation from a teacher's K top logits (t_ids int64 / t_logits [rows][K], K <= pv_distill_max_entries()): with p the
  * softmax of the row's teacher logits and q that of its logits, both at the temperature 1 / inv_temp,
  *   loss = scale / inv_temp^2 * sum over live rows of sum_j p_j (log p_j - log q[t_ids_j])
@@ -563,10 +567,10 @@ int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, 
 int pv_distill_max_entries(void);
 int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
                         int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
-                        float weight, int word, float* loss, float* save, float* psum, void* ws, void* stream);
+                        float weight, int word, float* loss, float* save, float* psum, void* dlogits, void* ws, void* stream);
 int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp,
-                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, void* dlogits,
-                        void* stream);
+                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, int ready,
+                        void* dlogits, void* stream);
 /* The same policy loss from log-probabilities (no entropy term, stats[3] = 0).  dlogp: n0 * n1 + 1 floats kept for the backward
  * call (the last one is the scale; NULL: no gradient wanted).  ws: pv_vocab_rows_ws_bytes(0). */
 int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,

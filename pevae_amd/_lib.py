@@ -148,13 +148,14 @@ SIGNATURES = {
     "pv_dropout_f32": (i32, [vp, i32, i32, i32, lng, lng, lng, lng, lng, f32, vp, vp, i32, vp, lng, lng, vp]),
     "pv_dropout_pack_bf16": (i32, [vp, i32, i32, i32, i32, lng, lng, lng, lng, lng, f32, vp, vp, i32, vp, i32, vp]),
     "pv_vocab_rows_ws_bytes": (sz, [lng]),
+    "pv_vocab_rows_one_pass": (i32, [i32, i32]),
     "pv_token_logp_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp]),
     "pv_token_logp_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp, vp]),
-    "pv_policy_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, i32, f32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),
-    "pv_policy_rows_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp]),
+    "pv_policy_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, i32, f32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp, vp]),
+    "pv_policy_rows_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, vp, vp]),
     "pv_distill_max_entries": (i32, []),
-    "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp]),
-    "pv_distill_rows_bwd": (i32, _ROWS + [f32, vp, i32, vp, vp, vp, vp, vp]),
+    "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp, vp]),
+    "pv_distill_rows_bwd": (i32, _ROWS + [f32, vp, i32, vp, vp, vp, i32, vp, vp]),
     "pv_policy_tokens_fwd": (i32, [vp, vp, i64, lng, i32, vp, vp, vp, i32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),
     "pv_policy_tokens_bwd": (i32, [vp, vp, lng, vp, vp]),
     "pv_preference_fwd": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, lng, i64, f32, f32, f32, vp, vp, vp, vp, vp]),

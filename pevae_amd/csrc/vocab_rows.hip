@@ -32,6 +32,7 @@ __device__ __forceinline__ uint32_t as_uint(float f) { return __builtin_bit_cast
 struct F32 {
   typedef float type;
   static constexpr int N = 4;
+  static __device__ __forceinline__ u32x4 nothing() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
   static __device__ __forceinline__ float up(float x) { return x; }
   static __device__ __forceinline__ float down(float x) { return x; }
   static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[4]) {
@@ -48,6 +49,7 @@ struct F32 {
 struct BF16 {
   typedef bf16_t type;
   static constexpr int N = 8;
+  static __device__ __forceinline__ u32x4 nothing() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
   static __device__ __forceinline__ float up(bf16_t x) { return bf2f(x); }
   static __device__ __forceinline__ bf16_t down(float x) { return f2bf(x); }
   static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
@@ -67,6 +69,7 @@ struct BF16 {
 struct F16 {
   typedef uint16_t type;
   static constexpr int N = 8;
+  static __device__ __forceinline__ u32x4 nothing() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
   static __device__ __forceinline__ float up(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
   static __device__ __forceinline__ uint16_t down(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
   static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
@@ -84,6 +87,8 @@ struct F16 {
   }
 };
 
+// the compiler forgets what it has unpacked from a piece: the packed form is what stays in registers
+__device__ __forceinline__ void keep_packed(u32x4& r) { asm volatile("" : "+v"(r)); }
 __device__ __forceinline__ u32x4 load_piece(const void* p) { return ((const piece_t*)p)->v; }
 __device__ __forceinline__ void store_piece(void* p, u32x4 v) { ((piece_t*)p)->v = v; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -120,6 +125,12 @@ __device__ __forceinline__ Stat wave_stat(Stat st, float k) {
   const float m = wave_max(st.m);
   rebase(st, finite_max(m), k);
   return {m, wave_sum(st.s), wave_sum(st.ex)};
+}
+
+// e (a + b x) for w = {m, a, b, -}
+__device__ __forceinline__ float slope(float z, const float4& w, float k) {
+  const float x = (z - w.x) * k, e = exp2_(x);
+  return w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
 }
 
 // x - ln(s) to about half a unit of the result: ln s = n ln2 + ln f with the two halves of ln2 kept apart, the rounding of
@@ -211,68 +222,55 @@ struct Teacher {
   float acc, zref;
   bool empty, bad;
 };
+struct TeacherList {         // of a row, in shared memory
+  int id[kTeacherMax];       // -1: no word of the vocabulary
+  float p[kTeacherMax], psum[kTeacherMax];
+};
 template <class E>
-__device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, long t, const typename E::type* row, int lane) {
-  float x[4], z[4], p[4];
-  int id[4];
-  float mx = -__builtin_inff();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = lane + 64 * i;
-    x[i] = -__builtin_inff();
-    id[i] = -1;
-    if (j < h.K) {
-      x[i] = load_teacher(h, t * h.K + j);
-      const int64_t w = h.ids[t * h.K + j];
-      id[i] = w >= 0 && w < a.V ? (int)w : -1;
-    }
-    mx = fmaxf(mx, x[i]);
+__device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, long t, const typename E::type* row, int lane,
+                                               TeacherList& l) {
+  float mx = -__builtin_inff(), nan = 0.f;         // fmaxf drops a NaN: the sum keeps it
+  for (int j = lane; j < h.K; j += 64) {
+    const float x = load_teacher(h, t * h.K + j);
+    const int64_t w = h.ids[t * h.K + j];
+    l.id[j] = w >= 0 && w < a.V ? (int)w : -1;
+    l.p[j] = x;
+    mx = fmaxf(mx, x);
+    nan += x != x ? x : 0.f;
   }
-  float nan = 0.f;                                 // fmaxf drops a NaN: the sum below keeps it
-#pragma unroll
-  for (int i = 0; i < 4; ++i) nan += x[i] != x[i] ? x[i] : 0.f;
   mx = wave_max(mx) + wave_sum(nan);
   Teacher r;
   r.empty = mx == -__builtin_inff();
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    z[i] = id[i] >= 0 ? E::up(row[id[i]]) : 0.f;
-    p[i] = x[i] == -__builtin_inff() ? 0.f : exp2_((x[i] - mx) * a.k);
-    sum += p[i];
+  float sum = 0.f, zr = -__builtin_inff(), bad = 0.f;
+  for (int j = lane; j < h.K; j += 64) {
+    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * a.k);
+    sum += p;
+    if (p > 0.f) {
+      if (l.id[j] < 0)
+        bad = 1.f;
+      else
+        zr = fmaxf(zr, E::up(row[l.id[j]]));
+    }
   }
   sum = wave_sum(sum);
-  const float inv = r.empty ? 0.f : 1.f / sum;
-  float zr = -__builtin_inff(), bad = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p[i] *= inv;
-    if (p[i] > 0.f) {
-      if (id[i] < 0) bad = 1.f;
-      zr = fmaxf(zr, z[i]);
-    }
-  }
   r.bad = wave_sum(bad) > 0.f || sum != sum;       // (a NaN or +inf among the teacher's logits)
   r.zref = finite_max(wave_max(zr));
+  const float inv = r.empty ? 0.f : 1.f / sum;
   float acc = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (p[i] > 0.f) acc += p[i] * (minus_log((x[i] - mx) * a.c, sum) - a.c * (z[i] - r.zref));
-  r.acc = wave_sum(acc);
-  float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int n = h.K - 64 * q < 64 ? h.K - 64 * q : 64;
-    for (int l = 0; l < n; ++l) {
-      const int w = __shfl(id[q], l);
-      const float pw = __shfl(p[q], l);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ps[i] += w == id[i] ? pw : 0.f;
-    }
+  for (int j = lane; j < h.K; j += 64) {
+    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * a.k) * inv;
+    if (p > 0.f && l.id[j] >= 0) acc += p * (minus_log((x - mx) * a.c, sum) - a.c * (E::up(row[l.id[j]]) - r.zref));
+    l.p[j] = p;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < h.K) h.psum[t * h.K + lane + 64 * i] = ps[i];
+  r.acc = wave_sum(acc);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the lanes read each other's entries
+  for (int j = lane; j < h.K; j += 64) {
+    const int id = l.id[j];
+    float ps = 0.f;
+    for (int q = 0; q < h.K; ++q) ps += l.id[q] == id ? l.p[q] : 0.f;
+    l.psum[j] = ps;
+    h.psum[t * h.K + j] = ps;
+  }
   return r;
 }
 
@@ -301,36 +299,35 @@ __device__ __forceinline__ void accumulate(Stat& st, const float (&z)[N], float 
   st = {m, s, ex};
 }
 
-// the row's loss terms and the coefficients of its gradient
+// the row's loss terms (stored by one thread, where `first`) and {m, a, b, d}, the coefficients of its gradient
 template <int HEAD>
-__device__ __forceinline__ void finish_row(const Rows& a, const Policy& hp, const Scale& sc, const Teacher& te, const FwdOut& o,
-                                           long t, Stat st, float zy, bool bad) {
+__device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, const Scale& sc, const Teacher& te, const FwdOut& o,
+                                             long t, Stat st, float zy, bool bad, bool first) {
   const float nan = __builtin_nanf("");
   const float inv = 1.f / st.s, ln2 = 0.69314718056f;
   if (st.m == kDead) st.m = nan;                   // a logit of +inf: no distribution
   if (HEAD == HEAD_TOKEN) {
-    const float H = -minus_log(st.ex * inv * ln2, st.s);
-    if (o.logp) o.logp[t] = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
-    if (o.ent) o.ent[t] = H;
-    if (o.save) o.save[t] = make_float4(bad ? nan : st.m, inv, st.ex * inv, 0.f);
+    if (first) {
+      o.logp[t] = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
+      if (o.ent) o.ent[t] = -minus_log(st.ex * inv * ln2, st.s);
+    }
+    return make_float4(bad ? nan : st.m, inv, st.ex * inv, 0.f);
   } else if (HEAD == HEAD_POLICY) {
     const float lp = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
     const float H = -minus_log(st.ex * inv * ln2, st.s);
     const PolicyTerm q = policy_term(hp, lp, hp.old_lp[t], hp.ref_lp ? hp.ref_lp[t] : 0.f, hp.adv[hp.adv_per_row ? t : (long)((uint32_t)t / (uint32_t)a.n1)]);
-    o.rowout[t] = make_float4(q.pg, q.k3, q.cut, H);
-    if (o.save) {
-      // d(loss)/d(log p[y]) = g, d(loss)/dH = h: dz_v = c (g [v = y] - p_v (g + h (log p_v + H)))
-      const float w = sc.get(), g = w * q.dlp, h = -w * hp.ent;
-      o.save[t] = make_float4(st.m, -a.c * inv * (g - h * ln2 * st.ex * inv), -a.c * inv * h * ln2, a.c * g);
-    }
+    if (first) o.rowout[t] = make_float4(q.pg, q.k3, q.cut, H);
+    // d(loss)/d(log p[y]) = g, d(loss)/dH = h: dz_v = c (g [v = y] - p_v (g + h (log p_v + H)))
+    const float w = sc.get(), g = w * q.dlp, h = -w * hp.ent;
+    return make_float4(st.m, -a.c * inv * (g - h * ln2 * st.ex * inv), -a.c * inv * h * ln2, a.c * g);
   } else {
     const float tau = 1.f / a.c;
-    const float loss = te.bad ? nan : te.acc + (a.c * (st.m - te.zref) - minus_log(0.f, st.s));
-    o.rowout[t] = make_float4(te.empty ? 0.f : tau * tau * loss, 0.f, 0.f, 0.f);
-    if (o.save) {
-      const float w = sc.get() * tau;             // tau^2 / tau
-      o.save[t] = make_float4(te.empty ? kDead : st.m, te.bad ? nan : w * inv, 0.f, -w);
+    if (first) {
+      const float loss = te.bad ? nan : te.acc + (a.c * (st.m - te.zref) - minus_log(0.f, st.s));
+      o.rowout[t] = make_float4(te.empty ? 0.f : tau * tau * loss, 0.f, 0.f, 0.f);
     }
+    const float w = sc.get() * tau;               // tau^2 / tau
+    return make_float4(te.empty ? kDead : st.m, te.bad ? nan : w * inv, 0.f, -w);
   }
 }
 
@@ -355,7 +352,8 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(Rows a, Policy hp, Distil
   const bool bad = HEAD != HEAD_DISTILL && (y < 0 || y >= a.V);
   const float zy = HEAD != HEAD_DISTILL && !bad ? E::up(row[y]) : 0.f;
   Teacher te = {0.f, 0.f, false, false};
-  if (HEAD == HEAD_DISTILL && wave == 0) te = teacher_row<E>(a, hd, t, row, lane);
+  __shared__ TeacherList list;
+  if (HEAD == HEAD_DISTILL && wave == 0) te = teacher_row<E>(a, hd, t, row, lane, list);
   Stat st = {-__builtin_inff(), 0.f, 0.f};
   const int full = a.V / E::N;
   for (int c0 = tid; c0 < full; c0 += 4 * 256) {
@@ -383,7 +381,133 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(Rows a, Policy hp, Distil
   if (wave != 0) return;
   st = lane < 4 ? part[lane] : Stat{-__builtin_inff(), 0.f, 0.f};
   st = wave_stat(st, a.k);
-  if (lane == 0) finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad);
+  if (lane == 0) {
+    const float4 w = finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad, true);
+    if (o.save) o.save[t] = w;
+  }
+}
+
+// Loss and gradient of a row in one pass: the row stays in the registers of its workgroup (CH pieces a thread) between its
+// statistics and its gradient, so that it is read once and its gradient written once; a forward and a backward pass over
+// memory would read it twice.  Each wave takes the maximum and the sums of its own elements; one exchange through shared
+// memory gives every wave the row's.
+template <class E, int HEAD, int NT, int CH>
+__global__ __launch_bounds__(NT) void rows_once_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o,
+                                                       typename E::type* __restrict__ grad) {
+  constexpr int W = NT / 64;
+  const long t = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int full = a.V / E::N, rest = full * E::N + tid;
+  typename E::type* out = grad + t * a.V;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  const int64_t y = a.labels ? a.labels[t] : -1;
+  if (a.labels && y == a.ignore) {
+    for (int i = tid; i < full; i += NT) store_piece(out + (long)i * E::N, zero);
+    if (rest < a.V) out[rest] = E::down(0.f);
+    if (tid == 0) {
+      o.rowout[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+      o.save[t] = make_float4(kDead, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
+  const typename E::type* row = row_of<E>(a, t);
+  u32x4 raw[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+    raw[i] = tid + i * NT < full ? load_piece(row + (long)(tid + i * NT) * E::N) : E::nothing();
+  const float zr = rest < a.V ? E::up(row[rest]) : -__builtin_inff();
+  const bool bad = HEAD == HEAD_POLICY && (y < 0 || y >= a.V);
+  const float zy = HEAD == HEAD_POLICY && !bad ? E::up(row[y]) : 0.f;
+  __shared__ Stat part[W];
+  __shared__ int flags[2];
+  __shared__ TeacherList list;
+  Teacher te = {0.f, 0.f, false, false};
+  if (HEAD == HEAD_DISTILL && wave == 0) {
+    te = teacher_row<E>(a, hd, t, row, lane, list);
+    if (lane == 0) {
+      flags[0] = te.empty;
+      flags[1] = te.bad;
+    }
+  }
+  Stat st = {zr, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    float z[E::N];
+    E::unpack(raw[i], z);
+#pragma unroll
+    for (int n = 0; n < E::N; ++n) st.m = fmaxf(st.m, z[n]);
+  }
+  st.m = wave_max(st.m);
+  const float mw = finite_max(st.m);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    float z[E::N];
+    keep_packed(raw[i]);
+    E::unpack(raw[i], z);
+#pragma unroll
+    for (int n = 0; n < E::N; ++n) {
+      const float x = (z[n] - mw) * a.k, e = exp2_(x);
+      st.s += e;
+      if (HEAD == HEAD_POLICY) st.ex += e * fmaxf(x, kFloorX);
+    }
+  }
+  {
+    const float x = (zr - mw) * a.k, e = exp2_(x);
+    st.s += e;
+    if (HEAD == HEAD_POLICY) st.ex += e * fmaxf(x, kFloorX);
+  }
+  st.s = wave_sum(st.s);
+  if (HEAD == HEAD_POLICY) st.ex = wave_sum(st.ex);
+  if (lane == 0) part[wave] = st;
+  __syncthreads();
+  st = part[lane & (W - 1)];                       // every group of W lanes holds all waves' parts
+  float m = st.m;
+#pragma unroll
+  for (int i = W / 2; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+  rebase(st, finite_max(m), a.k);
+  st.m = m;
+#pragma unroll
+  for (int i = W / 2; i > 0; i >>= 1) {
+    st.s += __shfl_xor(st.s, i);
+    if (HEAD == HEAD_POLICY) st.ex += __shfl_xor(st.ex, i);
+  }
+  if (HEAD == HEAD_DISTILL && wave != 0) {
+    te.empty = flags[0];
+    te.bad = flags[1];
+  }
+  const float4 w = finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad, tid == 0);
+  if (tid == 0) o.save[t] = w;
+  if (HEAD == HEAD_DISTILL && w.x == kDead) {
+    for (int i = tid; i < full; i += NT) store_piece(out + (long)i * E::N, zero);
+    if (rest < a.V) out[rest] = E::down(0.f);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int v = (tid + i * NT) * E::N;
+    if (tid + i * NT >= full) break;
+    float z[E::N];
+    keep_packed(raw[i]);
+    E::unpack(raw[i], z);
+#pragma unroll
+    for (int n = 0; n < E::N; ++n) {
+      z[n] = slope(z[n], w, a.k);
+      if (HEAD == HEAD_POLICY && v + n == (int)y) z[n] += w.w;
+    }
+    store_piece(out + v, E::pack(z));
+  }
+  if (rest < a.V) {
+    float d = slope(zr, w, a.k);
+    if (HEAD == HEAD_POLICY && rest == (int)y) d += w.w;
+    out[rest] = E::down(d);
+  }
+  if (HEAD == HEAD_DISTILL) {
+    __syncthreads();                               // the list's words are written again, after the sweep
+    for (int j = tid; j < hd.K; j += NT) {
+      const int id = list.id[j];
+      if (id >= 0) out[id] = E::down(slope(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
+    }
+  }
 }
 
 // ---- gradient: dz_v = g (e_v (a + b x_v) + d [v in the row's list]), pieces of rows dealt out to workgroups ----------------
@@ -392,6 +516,7 @@ struct Grad {
   const float *dlogp, *dent; // HEAD_TOKEN: upstream gradients a row
   const float* g;            // else: upstream gradient of the loss (device scalar)
   void* out;                 // [T][V]
+  int ready;                 // out holds the gradient for *g = 1 already
 };
 
 template <class E, int HEAD>
@@ -399,6 +524,7 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad
   const int tid = threadIdx.x;
   constexpr int kItem = 256 * 4 * E::N;            // elements of a row that a workgroup takes at a time
   const float up = HEAD == HEAD_TOKEN ? 1.f : *q.g;
+  if (HEAD != HEAD_TOKEN && q.ready && up == 1.f) return;
   for (long it = blockIdx.x; it < items; it += gridDim.x) {
     const long t = it / blocks_per_row;
     const int v0 = (int)(it - t * blocks_per_row) * kItem, v1 = a.V - v0 < kItem ? a.V : v0 + kItem;
@@ -439,16 +565,14 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad
       E::unpack(raw[i], z);
 #pragma unroll
       for (int n = 0; n < E::N; ++n) {
-        const float x = (z[n] - w.x) * a.k, e = exp2_(x);
-        z[n] = w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
+        z[n] = slope(z[n], w, a.k);
         if (HEAD != HEAD_DISTILL && v + n == y) z[n] += dy;
       }
       store_piece(out + v, E::pack(z));
     }
     const int rest = v0 + full * E::N + tid;
     if (rest < v1) {
-      const float x = (E::up(row[rest]) - w.x) * a.k, e = exp2_(x);
-      float d = w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
+      float d = slope(E::up(row[rest]), w, a.k);
       if (HEAD != HEAD_DISTILL && rest == y) d += dy;
       out[rest] = E::down(d);
     }
@@ -457,8 +581,7 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad
       if (tid < hd.K) {
         const int64_t id = hd.ids[t * hd.K + tid];
         if (id >= v0 && id < v1) {
-          const float e = exp2_((E::up(row[id]) - w.x) * a.k);
-          out[id] = E::down(e * w.y + dy * hd.psum[t * hd.K + tid]);
+          out[id] = E::down(slope(E::up(row[id]), w, a.k) + dy * hd.psum[t * hd.K + tid]);
         }
       }
     }
@@ -679,6 +802,41 @@ int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, co
   return PV_OK;
 }
 
+// pieces of a row that the one-pass kernel can hold, and its launch
+constexpr int kOncePieces = 1024 * 20;
+template <class E, int HEAD>
+int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad,
+                      hipStream_t st) {
+  const int pieces = a.V / E::N;
+  typename E::type* g = (typename E::type*)grad;
+#define PV_ONCE(NT, CH)                                                                                         \
+  if (pieces <= NT * CH) {                                                                                      \
+    rows_once_kernel<E, HEAD, NT, CH><<<dim3((unsigned)a.T), dim3(NT), 0, st>>>(a, hp, hd, sc, o, g);           \
+    PV_LAUNCH_CHECK("rows_once_kernel");                                                                        \
+    return PV_OK;                                                                                               \
+  }
+  PV_ONCE(64, 4)
+  PV_ONCE(256, 4)
+  PV_ONCE(512, 4)
+  PV_ONCE(512, 6)
+  PV_ONCE(512, 8)
+  PV_ONCE(1024, 6)
+  PV_ONCE(1024, 8)
+  PV_ONCE(1024, 12)
+  PV_ONCE(1024, 16)
+  PV_ONCE(1024, 20)
+#undef PV_ONCE
+  pv_set_error("rows_once_kernel: a row of %d words does not fit", a.V);
+  return PV_ERR_LIMIT;
+}
+template <int HEAD>
+int launch_once(int dtype, const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad,
+                hipStream_t st) {
+  if (dtype == PV_DTYPE_F32) return launch_once_typed<F32, HEAD>(a, hp, hd, sc, o, grad, st);
+  if (dtype == PV_DTYPE_BF16) return launch_once_typed<BF16, HEAD>(a, hp, hd, sc, o, grad, st);
+  return launch_once_typed<F16, HEAD>(a, hp, hd, sc, o, grad, st);
+}
+
 template <int HEAD>
 int launch_grad(int dtype, const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
   const int item = 256 * 4 * (dtype == PV_DTYPE_F32 ? 4 : 8);
@@ -724,6 +882,10 @@ size_t pv_vocab_rows_ws_bytes(long rows) {
   return rows < 0 ? 0 : (size_t)rows * sizeof(float4) + kSumGroups * sizeof(Sum5) + sizeof(float);
 }
 
+int pv_vocab_rows_one_pass(int dtype, int V) {
+  return V > 0 && V / (dtype == PV_DTYPE_F32 ? 4 : 8) <= kOncePieces;
+}
+
 int pv_token_logp_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                       int64_t ignore, float inv_temp, float* logp, float* entropy, float* save, void* stream) {
   const int rc = check_rows("pv_token_logp_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
@@ -742,18 +904,19 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && save && dlogits && (dlogp || dentropy), "pv_token_logp_bwd: null argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
-  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, dlogp, dentropy, nullptr, dlogits},
+  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, dlogp, dentropy, nullptr, dlogits, 0},
                                  (hipStream_t)stream);
 }
 
 int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                        int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
                        int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
-                       float* loss, float* stats, float* save, void* ws, void* stream) {
+                       float* loss, float* stats, float* save, void* dlogits, void* ws, void* stream) {
   const int rc = check_rows("pv_policy_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && old_logp && adv && loss && stats && ws, "pv_policy_rows_fwd: null argument");
   PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_rows_fwd: the clip range is empty");
+  PV_REQUIRE(!dlogits || (save && pv_vocab_rows_one_pass(dtype, V)), "pv_policy_rows_fwd: no gradient in the forward pass here");
   hipStream_t st = (hipStream_t)stream;
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
   float4* rowout = (float4*)ws;
@@ -766,18 +929,20 @@ int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, 
     sc.count = count;
   }
   const Policy hp = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, ent_coef};
-  const int r = launch_fwd<HEAD_POLICY, true>(dtype, a, hp, Distill{}, sc, FwdOut{nullptr, nullptr, rowout, (float4*)save}, st);
+  const FwdOut o = {nullptr, nullptr, rowout, (float4*)save};
+  const int r = dlogits ? launch_once<HEAD_POLICY>(dtype, a, hp, Distill{}, sc, o, dlogits, st)
+                        : launch_fwd<HEAD_POLICY, true>(dtype, a, hp, Distill{}, sc, o, st);
   if (r != PV_OK) return r;
   return launch_sum(rowout, tokens, ignore, a.T, part, Result{kl_coef, ent_coef, weight, word, loss, stats, nullptr}, st);
 }
 
 int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
-                       int64_t ignore, float inv_temp, const float* save, const float* g, void* dlogits, void* stream) {
+                       int64_t ignore, float inv_temp, const float* save, const float* g, int ready, void* dlogits, void* stream) {
   const int rc = check_rows("pv_policy_rows_bwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && save && g && dlogits, "pv_policy_rows_bwd: null argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
-  return launch_grad<HEAD_POLICY>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, g, dlogits},
+  return launch_grad<HEAD_POLICY>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, g, dlogits, ready},
                                   (hipStream_t)stream);
 }
 
@@ -785,13 +950,14 @@ int pv_distill_max_entries(void) { return kTeacherMax; }
 
 int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
                         int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
-                        float weight, int word, float* loss, float* save, float* psum, void* ws, void* stream) {
+                        float weight, int word, float* loss, float* save, float* psum, void* dlogits, void* ws, void* stream) {
   const int rc = check_rows("pv_distill_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(t_ids && t_logits && loss && psum && ws, "pv_distill_rows_fwd: null argument");
   PV_REQUIRE(t_dtype == PV_DTYPE_F32 || t_dtype == PV_DTYPE_BF16 || t_dtype == PV_DTYPE_F16,
              "pv_distill_rows_fwd: unknown teacher dtype %d", t_dtype);
   PV_REQUIRE(K > 0, "pv_distill_rows_fwd: no teacher entries");
+  PV_REQUIRE(!dlogits || (save && pv_vocab_rows_one_pass(dtype, V)), "pv_distill_rows_fwd: no gradient in the forward pass here");
   if (K > kTeacherMax) {
     pv_set_error("pv_distill_rows_fwd: %d teacher entries are beyond the limit of %d", K, kTeacherMax);
     return PV_ERR_LIMIT;
@@ -809,20 +975,22 @@ int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0,
     sc.count = count;
   }
   const Distill hd = {t_ids, t_logits, K, t_dtype, psum};
-  const int r = launch_fwd<HEAD_DISTILL, false>(dtype, a, Policy{}, hd, sc, FwdOut{nullptr, nullptr, rowout, (float4*)save}, st);
+  const FwdOut o = {nullptr, nullptr, rowout, (float4*)save};
+  const int r = dlogits ? launch_once<HEAD_DISTILL>(dtype, a, Policy{}, hd, sc, o, dlogits, st)
+                        : launch_fwd<HEAD_DISTILL, false>(dtype, a, Policy{}, hd, sc, o, st);
   if (r != PV_OK) return r;
   return launch_sum(rowout, labels, ignore, a.T, part, Result{0.f, 0.f, weight, word, loss, nullptr, nullptr}, st);
 }
 
 int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp,
-                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, void* dlogits,
-                        void* stream) {
+                        const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, int ready,
+                        void* dlogits, void* stream) {
   const int rc = check_rows("pv_distill_rows_bwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(t_ids && save && psum && g && dlogits && K > 0 && K <= kTeacherMax, "pv_distill_rows_bwd: bad argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, nullptr, 0, inv_temp);
   return launch_grad<HEAD_DISTILL>(dtype, a, Distill{t_ids, nullptr, K, 0, (float*)psum},
-                                   Grad{(const float4*)save, nullptr, nullptr, g, dlogits}, (hipStream_t)stream);
+                                   Grad{(const float4*)save, nullptr, nullptr, g, dlogits, ready}, (hipStream_t)stream);
 }
 
 int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,

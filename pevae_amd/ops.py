@@ -2767,6 +2767,21 @@ def _avg(avg_type, weight, sequences):
     raise ValueError("Unknown avg type")
 
 
+def _one_pass_grad(logits, want):
+    """The gradient's tensor where the forward pass writes it: rows that fit the kernel that holds them on chip."""
+    if want and _lib.load().pv_vocab_rows_one_pass(_ROW_DTYPES[logits.dtype], logits.shape[-1]):
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return None
+
+
+def _take_grad(ctx, x, shape):
+    """(gradient tensor, 1 if the forward pass has written it): a second backward pass gets a tensor of its own."""
+    d, ctx.grad = ctx.grad, None
+    if d is not None:
+        return d, 1
+    return torch.empty(shape, dtype=x.dtype, device=x.device), 0
+
+
 class TokenLogProbs(torch.autograd.Function):
     """log_softmax(logits * inv_temp)[token] and the entropy of a row; the log-softmax itself is never written."""
 
@@ -2826,11 +2841,13 @@ class DistillTopK(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
         psum = torch.empty((T, K), dtype=torch.float32, device=dev)
+        d = _one_pass_grad(logits, want_grad)
         ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
         _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, _p(ids), _p(t_logits),
-                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), _p(save), _p(psum), _p(ws))
+                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), _p(save), _p(psum), _p(d), _p(ws))
         if want_grad:
             ctx.save_for_backward(x, ids, save, psum)
+            ctx.grad = d
         ctx.meta = (inv_temp, K, logits.shape)
         return loss
 
@@ -2839,8 +2856,9 @@ class DistillTopK(torch.autograd.Function):
     def backward(ctx, g):
         x, ids, save, psum = ctx.saved_tensors
         inv_temp, K, shape = ctx.meta
-        d = torch.empty(shape, dtype=x.dtype, device=x.device)
-        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(save), _p(psum), _p(g.contiguous()), _p(d))
+        d, ready = _take_grad(ctx, x, shape)
+        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(save), _p(psum), _p(g.contiguous()), ready,
+                _p(d))
         return (d,) + (None,) * 8
 
 
@@ -2888,11 +2906,13 @@ class VocabPolicyLoss(torch.autograd.Function):
         dev, T = x.device, tokens.numel()
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
         save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
+        d = _one_pass_grad(logits, want_grad)
         ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
         _launch(dev, "pv_policy_rows_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(old), _p(ref), _p(adv),
-                int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), _p(save), _p(ws))
+                int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), _p(save), _p(d), _p(ws))
         if want_grad:
             ctx.save_for_backward(x, tokens, save)
+            ctx.grad = d
         ctx.meta = (ignore, inv_temp, logits.shape)
         ctx.mark_non_differentiable(stats)
         return loss, stats
@@ -2902,8 +2922,9 @@ class VocabPolicyLoss(torch.autograd.Function):
     def backward(ctx, g, _dstats):
         x, tokens, save = ctx.saved_tensors
         ignore, inv_temp, shape = ctx.meta
-        d = torch.empty(shape, dtype=x.dtype, device=x.device)
-        _launch(x.device, "pv_policy_rows_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(save), _p(g.contiguous()), _p(d))
+        d, ready = _take_grad(ctx, x, shape)
+        _launch(x.device, "pv_policy_rows_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(save), _p(g.contiguous()), ready,
+                _p(d))
         return (d,) + (None,) * 13
 
 

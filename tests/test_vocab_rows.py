@@ -84,10 +84,13 @@ def test_entry_points_refuse_on_the_host():
         assert b"pv_token_logp_fwd" in lib.pv_last_error()
     assert logp(n0=1 << 16, n1=1 << 15) == -3
     assert logp(V=(1 << 24) + 1) == -3
-    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, p, None) == -3
-    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, p, None) == -1
-    assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, p, None) == -1
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, None, p, None) == -3
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, None, p, None) == -1
+    assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, None, p, None) == -1
     assert lib.pv_policy_tokens_fwd(p, p, 0, 0, 4, p, None, p, 0, 0.8, 1.2, 0.0, 1.0, 0, p, p, p, p, None) == -1
     assert lib.pv_preference_fwd(None, None, None, 3, p, None, p, 3, 2, 0, 0.1, 0.0, 1.0, p, p, p, p, None) == -1
+    assert lib.pv_vocab_rows_one_pass(0, 81923) == 1 and lib.pv_vocab_rows_one_pass(0, 81924) == 0     # 20 480 pieces of 16 bytes
+    assert lib.pv_vocab_rows_one_pass(1, 163847) == 1 and lib.pv_vocab_rows_one_pass(2, 163848) == 0
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 81924, 81924, None, 0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, p, None) == -1
     assert lib.pv_distill_max_entries() == 256
     assert lib.pv_vocab_rows_ws_bytes(10) >= 160
