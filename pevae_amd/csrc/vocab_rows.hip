@@ -8,8 +8,10 @@
 // with a, b and the list known once the row's statistics are.  All statistics, sums and coefficients are fp32 or fp64;
 // only the gradient is rounded to the logits' type, once.
 //
-// The rows are read in 16-byte pieces whatever the address of a row is (odd vocabularies put rows at any element):
-// gfx950 takes unaligned global accesses.
+// Rows start at any element (an odd vocabulary puts every second row of a 16-bit type at an odd one), and are taken in 16-byte
+// pieces from the first aligned one on (of the gradient's row where one is written); the up to N - 1 elements before it and
+// behind the last piece go to one thread each.  gfx950 takes unaligned global accesses, so logits and gradient may be aligned
+// differently; pieces at odd 2-byte addresses cost 15 to 18 % (V = 20003 against 20002, bf16).
 #include "common.h"
 #include "../../include/pevae_hip.h"
 
@@ -31,7 +33,7 @@ __device__ __forceinline__ uint32_t as_uint(float f) { return __builtin_bit_cast
 
 struct F32 {
   typedef float type;
-  static constexpr int N = 4;
+  static constexpr int N = 4;              // elements of a piece
   static __device__ __forceinline__ u32x4 nothing() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
   static __device__ __forceinline__ float up(float x) { return x; }
   static __device__ __forceinline__ float down(float x) { return x; }
@@ -91,6 +93,21 @@ struct F16 {
 __device__ __forceinline__ void keep_packed(u32x4& r) { asm volatile("" : "+v"(r)); }
 __device__ __forceinline__ u32x4 load_piece(const void* p) { return ((const piece_t*)p)->v; }
 __device__ __forceinline__ void store_piece(void* p, u32x4 v) { ((piece_t*)p)->v = v; }
+// how a row of V elements at `p` splits: `head` elements, `full` pieces, then the rest; the element of thread tid outside the
+// pieces, or V where it has none
+template <class E>
+struct Split {
+  int head, full;
+  __device__ __forceinline__ Split(const void* p, int V) {
+    head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(typename E::type);
+    head = head < V ? head : V;
+    full = (V - head) / E::N;
+  }
+  __device__ __forceinline__ int edge(int tid, int V) const {
+    const int v = tid < head ? tid : tid + full * E::N;
+    return v < V ? v : V;
+  }
+};
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ float wave_max(float x) {
@@ -127,10 +144,24 @@ __device__ __forceinline__ Stat wave_stat(Stat st, float k) {
   return {m, wave_sum(st.s), wave_sum(st.ex)};
 }
 
-// e (a + b x) for w = {m, a, b, -}
+// e (a + b x) for w = {m, a, b, -}; B: b may differ from 0
+template <bool B>
 __device__ __forceinline__ float slope(float z, const float4& w, float k) {
   const float x = (z - w.x) * k, e = exp2_(x);
-  return w.z == 0.f ? e * w.y : e * (w.y + w.z * fmaxf(x, kFloorX));
+  return B ? e * (w.y + w.z * fmaxf(x, kFloorX)) : e * w.y;
+}
+// the gradient of one piece of a row whose first word is v; y: the word that gets d on top (none: negative)
+template <class E, bool B>
+__device__ __forceinline__ u32x4 slope_piece(u32x4 raw, int v, const float4& w, float k, int y, float d) {
+  float z[E::N];
+  E::unpack(raw, z);
+#pragma unroll
+  for (int n = 0; n < E::N; ++n) z[n] = slope<B>(z[n], w, k);
+  if ((unsigned)(y - v) < (unsigned)E::N) {        // one piece of the row
+#pragma unroll
+    for (int n = 0; n < E::N; ++n) z[n] += v + n == y ? d : 0.f;
+  }
+  return E::pack(z);
 }
 
 // x - ln(s) to about half a unit of the result: ln s = n ln2 + ln f with the two halves of ln2 kept apart, the rounding of
@@ -181,12 +212,23 @@ struct Scale {
   __device__ __forceinline__ float get() const { return count ? weight / fmaxf(*count, 1.f) : weight; }
 };
 
+__device__ __forceinline__ uint32_t sequence_of(const Rows& a, long t) { return (uint32_t)t / (uint32_t)a.n1; }  // t < 2^31
 template <class E>
 __device__ __forceinline__ const typename E::type* row_of(const Rows& a, long t) {
-  const uint32_t i = (uint32_t)t / (uint32_t)a.n1, j = (uint32_t)t - i * (uint32_t)a.n1;     // fewer than 2^31 rows
+  const uint32_t i = sequence_of(a, t), j = (uint32_t)t - i * (uint32_t)a.n1;
   return (const typename E::type*)a.logits + i * a.s0 + j * a.s1;
 }
 
+// what a row's loss needs besides its logits, asked for before the row itself: its latency passes behind the row's
+struct RowIn {
+  float old_lp, ref_lp, adv, scale;
+};
+template <int HEAD>
+__device__ __forceinline__ RowIn load_row_in(const Rows& a, const Policy& h, const Scale& sc, long t) {
+  if (HEAD == HEAD_TOKEN) return {0.f, 0.f, 0.f, 0.f};
+  if (HEAD == HEAD_DISTILL) return {0.f, 0.f, 0.f, sc.get()};
+  return {h.old_lp[t], h.ref_lp ? h.ref_lp[t] : 0.f, h.adv[h.adv_per_row ? t : (long)sequence_of(a, t)], sc.get()};
+}
 struct PolicyTerm {
   float pg, k3, cut, dlp;
 };
@@ -301,7 +343,7 @@ __device__ __forceinline__ void accumulate(Stat& st, const float (&z)[N], float 
 
 // the row's loss terms (stored by one thread, where `first`) and {m, a, b, d}, the coefficients of its gradient
 template <int HEAD>
-__device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, const Scale& sc, const Teacher& te, const FwdOut& o,
+__device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, const RowIn& in, const Teacher& te, const FwdOut& o,
                                              long t, Stat st, float zy, bool bad, bool first) {
   const float nan = __builtin_nanf("");
   const float inv = 1.f / st.s, ln2 = 0.69314718056f;
@@ -315,10 +357,10 @@ __device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, co
   } else if (HEAD == HEAD_POLICY) {
     const float lp = bad ? nan : minus_log((zy - st.m) * a.c, st.s);
     const float H = -minus_log(st.ex * inv * ln2, st.s);
-    const PolicyTerm q = policy_term(hp, lp, hp.old_lp[t], hp.ref_lp ? hp.ref_lp[t] : 0.f, hp.adv[hp.adv_per_row ? t : (long)((uint32_t)t / (uint32_t)a.n1)]);
+    const PolicyTerm q = policy_term(hp, lp, in.old_lp, in.ref_lp, in.adv);
     if (first) o.rowout[t] = make_float4(q.pg, q.k3, q.cut, H);
     // d(loss)/d(log p[y]) = g, d(loss)/dH = h: dz_v = c (g [v = y] - p_v (g + h (log p_v + H)))
-    const float w = sc.get(), g = w * q.dlp, h = -w * hp.ent;
+    const float w = in.scale, g = w * q.dlp, h = -w * hp.ent;
     return make_float4(st.m, -a.c * inv * (g - h * ln2 * st.ex * inv), -a.c * inv * h * ln2, a.c * g);
   } else {
     const float tau = 1.f / a.c;
@@ -326,186 +368,207 @@ __device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, co
       const float loss = te.bad ? nan : te.acc + (a.c * (st.m - te.zref) - minus_log(0.f, st.s));
       o.rowout[t] = make_float4(te.empty ? 0.f : tau * tau * loss, 0.f, 0.f, 0.f);
     }
-    const float w = sc.get() * tau;               // tau^2 / tau
+    const float w = in.scale * tau;               // tau^2 / tau
     return make_float4(te.empty ? kDead : st.m, te.bad ? nan : w * inv, 0.f, -w);
   }
 }
 
-template <class E, int HEAD, bool ENT>
-__global__ __launch_bounds__(256) void rows_fwd_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o) {
-  const long t = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// A row belongs to NT threads: a workgroup, or (NT = 64) one of the four waves of a workgroup, since launching a workgroup for
+// every short row costs more than the row (V = 1009, bf16: 1.3 ns a row).
+template <int NT>
+struct Place {
+  static constexpr int R = NT == 64 ? 4 : 1, W = NT / 64;       // rows of a workgroup, waves of a row
+  static_assert((W & (W - 1)) == 0, "waves are joined by halving");
+  static __device__ __forceinline__ long row() { return blockIdx.x * (long)R + (R > 1 ? threadIdx.x >> 6 : 0); }
+  static __device__ __forceinline__ int slot() { return R > 1 ? threadIdx.x >> 6 : 0; }
+  static __device__ __forceinline__ int tid() { return threadIdx.x & (NT - 1); }
+  static __device__ __forceinline__ void sync() {
+    if (W > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // the row's statistics for all its threads, from those of the threads
+  template <bool ENT>
+  static __device__ __forceinline__ Stat join(Stat st, float k, Stat (*part)[W]) {
+    st = wave_stat(st, k);
+    if (W == 1) return st;
+    if ((tid() & 63) == 0) part[0][tid() >> 6] = st;
+    sync();
+    st = part[0][threadIdx.x & (W - 1)];           // every group of W lanes holds all waves' parts
+    float m = st.m;
+#pragma unroll
+    for (int i = W / 2; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    rebase(st, finite_max(m), k);
+#pragma unroll
+    for (int i = W / 2; i > 0; i >>= 1) {
+      st.s += __shfl_xor(st.s, i);
+      if (ENT) st.ex += __shfl_xor(st.ex, i);
+    }
+    st.m = m;
+    return st;
+  }
+};
+
+template <int HEAD>
+__device__ __forceinline__ void dead_row(const FwdOut& o, long t) {
+  if (HEAD == HEAD_TOKEN) {
+    o.logp[t] = 0.f;
+    if (o.ent) o.ent[t] = 0.f;
+  } else {
+    o.rowout[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  if (o.save) o.save[t] = make_float4(kDead, 0.f, 0.f, 0.f);
+}
+
+// running statistics of a thread over the pieces first, first + step, ... below end of a row, four in flight
+template <class E, bool ENT>
+__device__ __forceinline__ void sweep_pieces(Stat& st, const typename E::type* row, int first, int step, int end, float k) {
+  for (int c = first; c < end; c += 4 * step) {
+    u32x4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = c + i * step < end ? load_piece(row + (long)(c + i * step) * E::N) : E::nothing();
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+      if (c + i * step < end) {                    // two pieces: the maximum moves, and the sums are rescaled, once for both
+        float f[E::N], z[2 * E::N];
+        E::unpack(raw[i], f);
+#pragma unroll
+        for (int n = 0; n < E::N; ++n) z[n] = f[n];
+        E::unpack(raw[i + 1], f);
+#pragma unroll
+        for (int n = 0; n < E::N; ++n) z[E::N + n] = f[n];
+        accumulate<2 * E::N, ENT>(st, z, k);
+      }
+  }
+}
+
+template <class E, int HEAD, bool ENT, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void rows_fwd_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o) {
+  typedef Place<NT> P;
+  const long t = P::row();
+  const int tid = P::tid();
+  if (P::R > 1 && t >= a.T) return;
   const int64_t y = a.labels ? a.labels[t] : -1;
   if (a.labels && y == a.ignore) {
-    if (tid == 0) {
-      if (HEAD == HEAD_TOKEN) {
-        if (o.logp) o.logp[t] = 0.f;
-        if (o.ent) o.ent[t] = 0.f;
-      } else {
-        o.rowout[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      if (o.save) o.save[t] = make_float4(kDead, 0.f, 0.f, 0.f);
-    }
+    if (tid == 0) dead_row<HEAD>(o, t);
     return;
   }
+  const RowIn in = load_row_in<HEAD>(a, hp, sc, t);
   const typename E::type* row = row_of<E>(a, t);
   const bool bad = HEAD != HEAD_DISTILL && (y < 0 || y >= a.V);
   const float zy = HEAD != HEAD_DISTILL && !bad ? E::up(row[y]) : 0.f;
   Teacher te = {0.f, 0.f, false, false};
-  __shared__ TeacherList list;
-  if (HEAD == HEAD_DISTILL && wave == 0) te = teacher_row<E>(a, hd, t, row, lane, list);
+  __shared__ TeacherList list[HEAD == HEAD_DISTILL ? P::R : 1];
+  __shared__ Stat part[1][P::W];
+  if (HEAD == HEAD_DISTILL && tid < 64) te = teacher_row<E>(a, hd, t, row, tid, list[P::slot()]);
   Stat st = {-__builtin_inff(), 0.f, 0.f};
-  const int full = a.V / E::N;
-  for (int c0 = tid; c0 < full; c0 += 4 * 256) {
-    u32x4 raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c0 + i * 256 < full) raw[i] = load_piece(row + (long)(c0 + i * 256) * E::N);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c0 + i * 256 < full) {
-        float z[E::N];
-        E::unpack(raw[i], z);
-        accumulate<E::N, ENT>(st, z, a.k);
-      }
-  }
-  const int rest = full * E::N + tid;
+  const Split<E> sp(row, a.V);
+  sweep_pieces<E, ENT>(st, row + sp.head, tid, NT, sp.full, a.k);
+  const int rest = sp.edge(tid, a.V);
   if (rest < a.V) {
-    float z[1] = {E::up(row[rest])};
+    const float z[1] = {E::up(row[rest])};
     accumulate<1, ENT>(st, z, a.k);
   }
-  st = wave_stat(st, a.k);
-  __shared__ Stat part[4];
-  if (lane == 0) part[wave] = st;
-  __syncthreads();
-  if (wave != 0) return;
-  st = lane < 4 ? part[lane] : Stat{-__builtin_inff(), 0.f, 0.f};
-  st = wave_stat(st, a.k);
-  if (lane == 0) {
-    const float4 w = finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad, true);
+  st = P::template join<ENT>(st, a.k, part);
+  if (tid == 0) {
+    const float4 w = finish_row<HEAD>(a, hp, in, te, o, t, st, zy, bad, true);
     if (o.save) o.save[t] = w;
   }
 }
 
-// Loss and gradient of a row in one pass: the row stays in the registers of its workgroup (CH pieces a thread) between its
-// statistics and its gradient, so that it is read once and its gradient written once; a forward and a backward pass over
-// memory would read it twice.  Each wave takes the maximum and the sums of its own elements; one exchange through shared
-// memory gives every wave the row's.
-template <class E, int HEAD, int NT, int CH>
-__global__ __launch_bounds__(NT) void rows_once_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o,
-                                                       typename E::type* __restrict__ grad) {
-  constexpr int W = NT / 64;
-  const long t = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int full = a.V / E::N, rest = full * E::N + tid;
+template <class E, bool B, int NT, int CH>
+__device__ __forceinline__ void write_once(u32x4 (&raw)[CH], typename E::type* out, int tid, const Split<E>& sp,
+                                           const float4& w, float k, int y, float d) {
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = tid + i * NT;
+    keep_packed(raw[i]);
+    const int v = sp.head + c * E::N;
+    if (c < sp.full) store_piece(out + v, slope_piece<E, B>(raw[i], v, w, k, y, d));
+  }
+}
+
+// Loss and gradient of a row in one pass: the row stays in its threads' registers (CH pieces each) between its statistics and
+// its gradient, so that it is read once and its gradient written once; a forward and a backward pass over memory would read it
+// twice.  Each thread runs its own maximum and sums while its pieces arrive; one exchange through shared memory gives every
+// wave the row's.  WAVES a SIMD bound the registers so that a CU holds several rows: while one waits for memory another one
+// computes.
+template <class E, int HEAD, int NT, int CH, int WAVES>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o,
+                                                                           typename E::type* __restrict__ grad) {
+  typedef Place<NT> P;
+  const long t = P::row();
+  const int tid = P::tid();
+  if (P::R > 1 && t >= a.T) return;
   typename E::type* out = grad + t * a.V;
+  const Split<E> sp(out, a.V);
+  const int full = sp.full, rest = sp.edge(tid, a.V);
   const u32x4 zero = {0u, 0u, 0u, 0u};
   const int64_t y = a.labels ? a.labels[t] : -1;
   if (a.labels && y == a.ignore) {
-    for (int i = tid; i < full; i += NT) store_piece(out + (long)i * E::N, zero);
+    for (int i = tid; i < full; i += NT) store_piece(out + sp.head + (long)i * E::N, zero);
     if (rest < a.V) out[rest] = E::down(0.f);
-    if (tid == 0) {
-      o.rowout[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-      o.save[t] = make_float4(kDead, 0.f, 0.f, 0.f);
-    }
+    if (tid == 0) dead_row<HEAD>(o, t);
     return;
   }
+  const RowIn in = load_row_in<HEAD>(a, hp, sc, t);
   const typename E::type* row = row_of<E>(a, t);
   u32x4 raw[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i)
-    raw[i] = tid + i * NT < full ? load_piece(row + (long)(tid + i * NT) * E::N) : E::nothing();
+    raw[i] = tid + i * NT < full ? load_piece(row + sp.head + (long)(tid + i * NT) * E::N) : E::nothing();
   const float zr = rest < a.V ? E::up(row[rest]) : -__builtin_inff();
   const bool bad = HEAD == HEAD_POLICY && (y < 0 || y >= a.V);
   const float zy = HEAD == HEAD_POLICY && !bad ? E::up(row[y]) : 0.f;
-  __shared__ Stat part[W];
+  __shared__ Stat part[1][P::W];
   __shared__ int flags[2];
-  __shared__ TeacherList list;
+  __shared__ TeacherList lists[HEAD == HEAD_DISTILL ? P::R : 1];
+  TeacherList& list = lists[HEAD == HEAD_DISTILL ? P::slot() : 0];
   Teacher te = {0.f, 0.f, false, false};
-  if (HEAD == HEAD_DISTILL && wave == 0) {
-    te = teacher_row<E>(a, hd, t, row, lane, list);
-    if (lane == 0) {
+  if (HEAD == HEAD_DISTILL && tid < 64) {
+    te = teacher_row<E>(a, hd, t, row, tid, list);
+    if (P::W > 1 && tid == 0) {
       flags[0] = te.empty;
       flags[1] = te.bad;
     }
   }
-  Stat st = {zr, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    float z[E::N];
-    E::unpack(raw[i], z);
-#pragma unroll
-    for (int n = 0; n < E::N; ++n) st.m = fmaxf(st.m, z[n]);
-  }
-  st.m = wave_max(st.m);
-  const float mw = finite_max(st.m);
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    float z[E::N];
-    keep_packed(raw[i]);
-    E::unpack(raw[i], z);
-#pragma unroll
-    for (int n = 0; n < E::N; ++n) {
-      const float x = (z[n] - mw) * a.k, e = exp2_(x);
-      st.s += e;
-      if (HEAD == HEAD_POLICY) st.ex += e * fmaxf(x, kFloorX);
-    }
-  }
+  constexpr bool ENT = HEAD == HEAD_POLICY;
+  Stat st = {-__builtin_inff(), 0.f, 0.f};
   {
-    const float x = (zr - mw) * a.k, e = exp2_(x);
-    st.s += e;
-    if (HEAD == HEAD_POLICY) st.ex += e * fmaxf(x, kFloorX);
+    const float z[1] = {zr};
+    accumulate<1, ENT>(st, z, a.k);
   }
-  st.s = wave_sum(st.s);
-  if (HEAD == HEAD_POLICY) st.ex = wave_sum(st.ex);
-  if (lane == 0) part[wave] = st;
-  __syncthreads();
-  st = part[lane & (W - 1)];                       // every group of W lanes holds all waves' parts
-  float m = st.m;
 #pragma unroll
-  for (int i = W / 2; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-  rebase(st, finite_max(m), a.k);
-  st.m = m;
-#pragma unroll
-  for (int i = W / 2; i > 0; i >>= 1) {
-    st.s += __shfl_xor(st.s, i);
-    if (HEAD == HEAD_POLICY) st.ex += __shfl_xor(st.ex, i);
-  }
-  if (HEAD == HEAD_DISTILL && wave != 0) {
+  for (int i = 0; i < CH; ++i)
+    if (tid + i * NT < full) {
+      float z[E::N];
+      E::unpack(raw[i], z);
+      accumulate<E::N, ENT>(st, z, a.k);
+    }
+  st = P::template join<ENT>(st, a.k, part);
+  if (HEAD == HEAD_DISTILL && P::W > 1) {
     te.empty = flags[0];
     te.bad = flags[1];
   }
-  const float4 w = finish_row<HEAD>(a, hp, sc, te, o, t, st, zy, bad, tid == 0);
+  const float4 w = finish_row<HEAD>(a, hp, in, te, o, t, st, zy, bad, tid == 0);
   if (tid == 0) o.save[t] = w;
   if (HEAD == HEAD_DISTILL && w.x == kDead) {
-    for (int i = tid; i < full; i += NT) store_piece(out + (long)i * E::N, zero);
+    for (int i = tid; i < full; i += NT) store_piece(out + sp.head + (long)i * E::N, zero);
     if (rest < a.V) out[rest] = E::down(0.f);
     return;
   }
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int v = (tid + i * NT) * E::N;
-    if (tid + i * NT >= full) break;
-    float z[E::N];
-    keep_packed(raw[i]);
-    E::unpack(raw[i], z);
-#pragma unroll
-    for (int n = 0; n < E::N; ++n) {
-      z[n] = slope(z[n], w, a.k);
-      if (HEAD == HEAD_POLICY && v + n == (int)y) z[n] += w.w;
-    }
-    store_piece(out + v, E::pack(z));
-  }
-  if (rest < a.V) {
-    float d = slope(zr, w, a.k);
-    if (HEAD == HEAD_POLICY && rest == (int)y) d += w.w;
-    out[rest] = E::down(d);
-  }
+  const int yy = HEAD == HEAD_POLICY ? (int)y : -1;
+  if (HEAD == HEAD_POLICY && w.z != 0.f)
+    write_once<E, true, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
+  else
+    write_once<E, false, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
+  if (rest < a.V) out[rest] = E::down(slope<HEAD == HEAD_POLICY>(zr, w, a.k) + (rest == yy ? w.w : 0.f));
   if (HEAD == HEAD_DISTILL) {
-    __syncthreads();                               // the list's words are written again, after the sweep
+    P::sync();                                     // the list's words are written again, after the sweep
     for (int j = tid; j < hd.K; j += NT) {
       const int id = list.id[j];
-      if (id >= 0) out[id] = E::down(slope(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
+      if (id >= 0) out[id] = E::down(slope<false>(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
     }
   }
 }
@@ -519,17 +582,37 @@ struct Grad {
   int ready;                 // out holds the gradient for *g = 1 already
 };
 
-template <class E, int HEAD>
-__global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad q, int blocks_per_row, long items) {
-  const int tid = threadIdx.x;
-  constexpr int kItem = 256 * 4 * E::N;            // elements of a row that a workgroup takes at a time
+// the pieces c, c + NT, ... below end of a row, four in flight
+template <class E, bool B, int NT>
+__device__ __forceinline__ void sweep_grad(const typename E::type* row, typename E::type* out, int head, int c, int end,
+                                           const float4& w, float k, int y, float d) {
+  for (; c < end; c += 4 * NT) {
+    u32x4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i * NT < end) raw[i] = load_piece(row + head + (long)(c + i * NT) * E::N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = head + (c + i * NT) * E::N;
+      if (c + i * NT < end) store_piece(out + v, slope_piece<E, B>(raw[i], v, w, k, y, d));
+    }
+  }
+}
+
+// NT threads (as above) take a row, or one of `blocks` equal shares of its pieces.
+template <class E, int HEAD, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, 8) void rows_grad_kernel(Rows a, Distill hd, Grad q, int blocks, long items) {
+  typedef Place<NT> P;
+  const int tid = P::tid();
   const float up = HEAD == HEAD_TOKEN ? 1.f : *q.g;
   if (HEAD != HEAD_TOKEN && q.ready && up == 1.f) return;
-  for (long it = blockIdx.x; it < items; it += gridDim.x) {
-    const long t = it / blocks_per_row;
-    const int v0 = (int)(it - t * blocks_per_row) * kItem, v1 = a.V - v0 < kItem ? a.V : v0 + kItem;
-    typename E::type* out = (typename E::type*)q.out + t * a.V;
-    const int full = (v1 - v0) / E::N;             // a multiple of the piece except at the row's end
+  for (long it = P::row(); it < items; it += gridDim.x * (long)P::R) {
+    const uint32_t t = (uint32_t)it / (uint32_t)blocks, share = (uint32_t)it - t * (uint32_t)blocks;   // items < 2^32
+    typename E::type* out = (typename E::type*)q.out + (long)t * a.V;
+    const Split<E> sp(out, a.V);
+    const int each = (sp.full + blocks - 1) / blocks, c0 = (int)share * each;
+    const int c1 = c0 + each < sp.full ? c0 + each : sp.full;
+    const int rest = share == 0 ? sp.edge(tid, a.V) : a.V;      // the first share has the edges
     float4 w = q.save[t];
     float dy = 0.f;
     int y = -1;
@@ -548,42 +631,26 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(Rows a, Distill hd, Grad
     }
     if (w.x == kDead) {
       const u32x4 zero = {0u, 0u, 0u, 0u};
-      for (int i = tid; i < full; i += 256) store_piece(out + v0 + (long)i * E::N, zero);
-      if (v0 + full * E::N + tid < v1) out[v0 + full * E::N + tid] = E::down(0.f);
+      for (int c = c0 + tid; c < c1; c += NT) store_piece(out + sp.head + (long)c * E::N, zero);
+      if (rest < a.V) out[rest] = E::down(0.f);
       continue;
     }
     const typename E::type* row = row_of<E>(a, t);
-    u32x4 raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (tid + i * 256 < full) raw[i] = load_piece(row + v0 + (long)(tid + i * 256) * E::N);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (tid + i * 256 >= full) break;
-      const int v = v0 + (tid + i * 256) * E::N;
-      float z[E::N];
-      E::unpack(raw[i], z);
-#pragma unroll
-      for (int n = 0; n < E::N; ++n) {
-        z[n] = slope(z[n], w, a.k);
-        if (HEAD != HEAD_DISTILL && v + n == y) z[n] += dy;
-      }
-      store_piece(out + v, E::pack(z));
-    }
-    const int rest = v0 + full * E::N + tid;
-    if (rest < v1) {
-      float d = slope(E::up(row[rest]), w, a.k);
-      if (HEAD != HEAD_DISTILL && rest == y) d += dy;
-      out[rest] = E::down(d);
-    }
+    if (HEAD != HEAD_DISTILL && w.z != 0.f)
+      sweep_grad<E, true, NT>(row, out, sp.head, c0 + tid, c1, w, a.k, y, dy);
+    else
+      sweep_grad<E, false, NT>(row, out, sp.head, c0 + tid, c1, w, a.k, y, dy);
+    if (rest < a.V) out[rest] = E::down(slope<HEAD != HEAD_DISTILL>(E::up(row[rest]), w, a.k) + (rest == y ? dy : 0.f));
     if (HEAD == HEAD_DISTILL) {
-      __syncthreads();                             // the list's words are written again, after the sweep
-      if (tid < hd.K) {
-        const int64_t id = hd.ids[t * hd.K + tid];
-        if (id >= v0 && id < v1) {
-          out[id] = E::down(slope(E::up(row[id]), w, a.k) + dy * hd.psum[t * hd.K + tid]);
-        }
+      P::sync();                                   // the list's words are written again, after the sweep
+      for (int j = tid; j < hd.K; j += NT) {
+        const int64_t id = hd.ids[(long)t * hd.K + j];
+        if (id < 0 || id >= a.V) continue;
+        const int piece = (int)id - sp.head;       // of this share: its pieces, and the edges with the first
+        const bool mine = piece < 0 || piece >= sp.full * E::N ? share == 0 : piece >= c0 * E::N && piece < c1 * E::N;
+        if (mine) out[id] = E::down(slope<false>(E::up(row[id]), w, a.k) + dy * hd.psum[(long)t * hd.K + j]);
       }
+      P::sync();
     }
   }
 }
@@ -601,11 +668,13 @@ __device__ __forceinline__ void block_sum(double (&v)[5], double (*sh)[5]) {
     if (lane == 0) sh[wave][i] = v[i];
   }
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int i = 0; i < 5; ++i) {
-      v[i] = sh[0][i];
-      for (int w = 1; w < waves; ++w) v[i] += sh[w][i];
-    }
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    v[i] = lane < waves ? sh[lane][i] : 0.0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v[i] += __shfl_xor(v[i], o);
+  }
 }
 // what becomes of the sums of {pg, k3, cut, H, live}
 struct Result {
@@ -628,13 +697,24 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float4* __restrict
                                                         int64_t ignore, long T, Sum5* __restrict__ part, Result r) {
   __shared__ double sh[16][5];
   double v[5] = {0, 0, 0, 0, 0};
-  for (long t = blockIdx.x * 1024L + threadIdx.x; t < T; t += gridDim.x * 1024L) {
-    const float4 q = rows[t];
-    v[0] += q.x;
-    v[1] += q.y;
-    v[2] += q.z;
-    v[3] += q.w;
-    v[4] += !labels || labels[t] != ignore ? 1.0 : 0.0;
+  const long step = gridDim.x * 1024L;
+  for (long t0 = blockIdx.x * 1024L + threadIdx.x; t0 < T; t0 += 8 * step) {
+    float4 q[8];
+    int64_t y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {                  // eight rows in flight
+      const long t = t0 + i * step;
+      q[i] = t < T ? rows[t] : make_float4(0.f, 0.f, 0.f, 0.f);
+      y[i] = t < T && labels ? labels[t] : ignore;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[0] += q[i].x;
+      v[1] += q[i].y;
+      v[2] += q[i].z;
+      v[3] += q[i].w;
+      v[4] += labels ? y[i] != ignore : t0 + i * step < T;
+    }
   }
   block_sum(v, sh);
   if (threadIdx.x == 0) {
@@ -664,14 +744,23 @@ __global__ __launch_bounds__(1024) void count_live_kernel(const int64_t* __restr
                                                           float* __restrict__ part, float* __restrict__ out) {
   __shared__ int sh[16];
   int n = 0;
-  for (long t = blockIdx.x * 1024L + threadIdx.x; t < T; t += gridDim.x * 1024L) n += labels[t] != ignore ? 1 : 0;
+  const long step = gridDim.x * 1024L;
+  for (long t0 = blockIdx.x * 1024L + threadIdx.x; t0 < T; t0 += 8 * step) {
+    int64_t y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = t0 + i * step < T ? labels[t0 + i * step] : ignore;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += y[i] != ignore ? 1 : 0;
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) n += sh[w];
-    (gridDim.x > 1 ? part[blockIdx.x] : out[0]) = (float)n;
+  if (threadIdx.x < 64) {
+    n = threadIdx.x < 16 ? sh[threadIdx.x] : 0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    if (threadIdx.x == 0) (gridDim.x > 1 ? part[blockIdx.x] : out[0]) = (float)n;
   }
 }
 __global__ __launch_bounds__(256) void add_counts_kernel(const float* __restrict__ part, int n, float* __restrict__ out) {
@@ -789,42 +878,61 @@ Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, con
   return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore};
 }
 
-template <int HEAD, bool ENT>
-int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
-  const dim3 grid((unsigned)a.T), block(256);
-  if (dtype == PV_DTYPE_F32)
-    rows_fwd_kernel<F32, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
-  else if (dtype == PV_DTYPE_BF16)
-    rows_fwd_kernel<BF16, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
-  else
-    rows_fwd_kernel<F16, HEAD, ENT><<<grid, block, 0, st>>>(a, hp, hd, sc, o);
+inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
+
+template <class E, int HEAD, bool ENT>
+int launch_fwd_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
+  const int pieces = a.V / E::N;
+  if (pieces <= 512)
+    rows_fwd_kernel<E, HEAD, ENT, 64><<<dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st>>>(a, hp, hd, sc, o);
+  else if (pieces <= 2048 || a.T >= 512)
+    rows_fwd_kernel<E, HEAD, ENT, 256><<<dim3((unsigned)a.T), dim3(256), 0, st>>>(a, hp, hd, sc, o);
+  else                                             // few long rows: a whole CU for each
+    rows_fwd_kernel<E, HEAD, ENT, 1024><<<dim3((unsigned)a.T), dim3(1024), 0, st>>>(a, hp, hd, sc, o);
   PV_LAUNCH_CHECK("rows_fwd_kernel");
   return PV_OK;
 }
+template <int HEAD, bool ENT>
+int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
+  if (dtype == PV_DTYPE_F32) return launch_fwd_typed<F32, HEAD, ENT>(a, hp, hd, sc, o, st);
+  if (dtype == PV_DTYPE_BF16) return launch_fwd_typed<BF16, HEAD, ENT>(a, hp, hd, sc, o, st);
+  return launch_fwd_typed<F16, HEAD, ENT>(a, hp, hd, sc, o, st);
+}
 
-// pieces of a row that the one-pass kernel can hold, and its launch
-constexpr int kOncePieces = 1024 * 20;
+// The one-pass kernel takes the fewest threads that can hold a row: fewer threads with more pieces each keep more rows of a CU
+// in flight.  Rates of live reads and writes (policy loss, TB/s): V = 1009, bf16: 64 x 4 3.1, 128 x 4 2.5; V = 5003, bf16:
+// 128 x 8 4.0, 256 x 4 3.7, 512 x 2 2.7; V = 20004, bf16: 512 x 6 4.8, 1024 x 4 3.8; V = 20004, fp32: 1024 x 6 5.3, 512 x 10 4.9.
+// Beyond 8 pieces a thread of a full CU the threads get more registers and a CU fewer rows: V = 80000, bf16: 512 x 20 (two
+// rows) 4.8, 1024 x 12 (one row) 4.2; V = 131071, bf16: 1024 x 16 3.9, which still beats two passes over memory (2.4).  Keeping
+// part of such rows in shared memory to hold two of them gained nothing (512 x 23 + 9: 3.6, its registers spill).
+constexpr int kOncePieces = 1024 * 20;            // of a row that the one-pass kernel holds
 template <class E, int HEAD>
 int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad,
                       hipStream_t st) {
   const int pieces = a.V / E::N;
   typename E::type* g = (typename E::type*)grad;
-#define PV_ONCE(NT, CH)                                                                                         \
+#define PV_ONCE(NT, CH, WAVES)                                                                                  \
   if (pieces <= NT * CH) {                                                                                      \
-    rows_once_kernel<E, HEAD, NT, CH><<<dim3((unsigned)a.T), dim3(NT), 0, st>>>(a, hp, hd, sc, o, g);           \
+    typedef Place<NT> P;                                                                                        \
+    rows_once_kernel<E, HEAD, NT, CH, WAVES>                                                                    \
+        <<<dim3((unsigned)((a.T + P::R - 1) / P::R)), dim3(NT * P::R), 0, st>>>(a, hp, hd, sc, o, g);            \
     PV_LAUNCH_CHECK("rows_once_kernel");                                                                        \
     return PV_OK;                                                                                               \
   }
-  PV_ONCE(64, 4)
-  PV_ONCE(256, 4)
-  PV_ONCE(512, 4)
-  PV_ONCE(512, 6)
-  PV_ONCE(512, 8)
-  PV_ONCE(1024, 6)
-  PV_ONCE(1024, 8)
-  PV_ONCE(1024, 12)
-  PV_ONCE(1024, 16)
-  PV_ONCE(1024, 20)
+  PV_ONCE(64, 2, 8)
+  PV_ONCE(64, 4, 8)
+  PV_ONCE(64, 8, 6)
+  PV_ONCE(128, 8, 7)
+  PV_ONCE(256, 6, 8)
+  PV_ONCE(256, 8, 7)
+  PV_ONCE(512, 6, 8)
+  PV_ONCE(512, 8, 6)
+  PV_ONCE(1024, 6, 8)
+  PV_ONCE(1024, 8, 8)
+  PV_ONCE(512, 20, 4)
+  PV_ONCE(1024, 12, 4)
+  PV_ONCE(1024, 16, 4)
+  PV_ONCE(1024, 20, 4)
 #undef PV_ONCE
   pv_set_error("rows_once_kernel: a row of %d words does not fit", a.V);
   return PV_ERR_LIMIT;
@@ -837,20 +945,25 @@ int launch_once(int dtype, const Rows& a, const Policy& hp, const Distill& hd, c
   return launch_once_typed<F16, HEAD>(a, hp, hd, sc, o, grad, st);
 }
 
-template <int HEAD>
-int launch_grad(int dtype, const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
-  const int item = 256 * 4 * (dtype == PV_DTYPE_F32 ? 4 : 8);
-  const int blocks = cdiv(a.V, item);
-  const long items = a.T * blocks;
-  const dim3 grid((unsigned)(items < 4096 ? items : 4096)), block(256);
-  if (dtype == PV_DTYPE_F32)
-    rows_grad_kernel<F32, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
-  else if (dtype == PV_DTYPE_BF16)
-    rows_grad_kernel<BF16, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
-  else
-    rows_grad_kernel<F16, HEAD><<<grid, block, 0, st>>>(a, hd, q, blocks, items);
+template <class E, int HEAD>
+int launch_grad_typed(const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
+  const int pieces = a.V / E::N;
+  if (pieces <= 512) {                             // a wave a row
+    const long quads = (a.T + 3) / 4;
+    rows_grad_kernel<E, HEAD, 64><<<dim3((unsigned)(quads < 2048 ? quads : 2048)), dim3(256), 0, st>>>(a, hd, q, 1, a.T);
+  } else {
+    const int blocks = cdiv(pieces, 256 * 4);
+    const long items = a.T * blocks;
+    rows_grad_kernel<E, HEAD, 256><<<dim3((unsigned)(items < 2048 ? items : 2048)), dim3(256), 0, st>>>(a, hd, q, blocks, items);
+  }
   PV_LAUNCH_CHECK("rows_grad_kernel");
   return PV_OK;
+}
+template <int HEAD>
+int launch_grad(int dtype, const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
+  if (dtype == PV_DTYPE_F32) return launch_grad_typed<F32, HEAD>(a, hd, q, st);
+  if (dtype == PV_DTYPE_BF16) return launch_grad_typed<BF16, HEAD>(a, hd, q, st);
+  return launch_grad_typed<F16, HEAD>(a, hd, q, st);
 }
 
 int launch_count(const int64_t* labels, int64_t ignore, long T, float* part, float* out, hipStream_t st) {
@@ -878,12 +991,13 @@ int launch_sum(const float4* rows, const int64_t* labels, int64_t ignore, long T
 
 extern "C" {
 
+// {the rows' terms, the sums' parts, the count}
 size_t pv_vocab_rows_ws_bytes(long rows) {
   return rows < 0 ? 0 : (size_t)rows * sizeof(float4) + kSumGroups * sizeof(Sum5) + sizeof(float);
 }
 
 int pv_vocab_rows_one_pass(int dtype, int V) {
-  return V > 0 && V / (dtype == PV_DTYPE_F32 ? 4 : 8) <= kOncePieces;
+  return V > 0 && pieces_of(dtype, V) <= kOncePieces;
 }
 
 int pv_token_logp_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
@@ -1002,7 +1116,7 @@ int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignor
   const long T = n0 * (long)n1;
   const Policy h = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, 0.f};
   const Result r = {kl_coef, 0.f, weight, word, loss, stats, dlogp ? dlogp + T : nullptr};
-  const long want = (T + 1023) / 1024;
+  const long want = (T + 255) / 256;
   const int g = (int)(want > kSumGroups ? kSumGroups : want);
   policy_tokens_kernel<<<dim3(g), dim3(256), 0, st>>>(logp, tokens, ignore, T, n1, h, dlogp, (Sum5*)ws, r);
   PV_LAUNCH_CHECK("policy_tokens_kernel");

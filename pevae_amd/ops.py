@@ -2686,12 +2686,13 @@ _NO_INDEX = -(1 << 63)           # an ignore index that no label has
 
 
 def _launch(dev, name, *args):
-    """One C call on `dev`'s current stream, whatever the current device is."""
+    """One C call on `dev`'s current stream, whatever the current device is.  (The raw handle: the Stream object around it
+    costs more than the launch of a small kernel.)"""
     if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def _same_device(*ts):
@@ -2713,7 +2714,7 @@ def _constant(name, t, shape):
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
     if not t.dtype.is_floating_point:
         raise ValueError("%s must be floating point (got %s)" % (name, t.dtype))
-    return t.detach().to(torch.float32).contiguous()
+    return t.detach().to(torch.float32).contiguous() if t.dtype != torch.float32 or not t.is_contiguous() else t
 
 
 def _index(name, t, shape):
@@ -2721,7 +2722,7 @@ def _index(name, t, shape):
         raise ValueError("%s must be int64 or int32 (got %s)" % (name, t.dtype))
     if tuple(t.shape) != tuple(shape):
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    return t.to(torch.int64).contiguous()
+    return t.to(torch.int64).contiguous() if t.dtype != torch.int64 or not t.is_contiguous() else t
 
 
 def _check_rows(logits):

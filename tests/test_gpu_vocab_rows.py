@@ -164,36 +164,39 @@ def test_tokens_that_name_no_word(dev):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strides_and_shapes(dev, dtype):
-    """The same rows in any layout give the same bits."""
+    """The same rows in any layout and at any alignment (which moves the order of the sums)."""
     from pevae_amd import ops
     B, L, V = 3, 5, 1001
     base = make((B, L, V), dtype, dev, 9)
     y = labels_of((B, L), V, dev, 10, dead=0.2)
     up = make((B, L), torch.float32, dev, 11)
+    p, lq = softmax64(base, 1.0)
+    live = y != -7
+    zero = torch.zeros(B, L, dtype=torch.float64, device=dev)
+    want = torch.where(live, lq.gather(-1, y.clamp(min=0)[..., None])[..., 0], zero)
+    dwant, dmag = rows_grad64(p, lq, zero, torch.where(live, y, torch.full_like(y, -1)), torch.where(live, up.double(), zero), zero, 1.0)
 
-    def run(x, tokens=y, g=up):
+    def check(x, name, pick=lambda t: t):
         x = x.detach().requires_grad_()
-        lp = ops.token_logprobs(x, tokens, ignore_index=-7)
-        d, = torch.autograd.grad(lp, x, g)
-        return lp.detach(), d
+        lp = ops.token_logprobs(x, pick(y), ignore_index=-7)
+        d, = torch.autograd.grad(lp, x, pick(up))
+        assert lp.shape == x.shape[:-1] and d.shape == x.shape
+        close(lp, pick(want), 1 + pick(want).abs(), name)
+        close(d, pick(dwant).reshape(x.shape), pick(dmag).reshape(x.shape), name + " gradient")
 
-    want, dwant = run(base)
-    padded = torch.full((B, L, 1030), float("nan"), dtype=dtype, device=dev)
-    padded[..., 3:3 + V] = base
-    time_major = base.transpose(0, 1).contiguous().transpose(0, 1)
-    word_major = base.permute(2, 0, 1).contiguous().permute(1, 2, 0)
-    flat = torch.zeros(B * L * V + 1, dtype=dtype, device=dev)
-    flat[1:] = base.reshape(-1)
-    for name, x in (("padded, odd start", padded[..., 3:3 + V]), ("time major", time_major), ("word major", word_major),
-                    ("odd start", flat[1:].view(B, L, V))):
-        lp, d = run(x)
-        assert torch.equal(lp, want) and torch.equal(d, dwant), name
-    lp, d = run(base.view(B * L, V), y.view(-1), up.view(-1))
-    assert torch.equal(lp.view(B, L), want) and torch.equal(d.view(B, L, V), dwant)
-    lp, d = run(base.view(B, 1, L, 1, V), y.view(B, 1, L, 1), up.view(B, 1, L, 1))
-    assert torch.equal(lp.view(B, L), want) and torch.equal(d.view(B, L, V), dwant)
-    lp, d = run(base[0, 0], y[0, 0], up[0, 0])
-    assert lp.shape == () and torch.equal(lp, want[0, 0]) and torch.equal(d, dwant[0, 0])
+    check(base, "contiguous")
+    for start in range(9):
+        padded = torch.full((B, L, 1030), float("nan"), dtype=dtype, device=dev)
+        padded[..., start:start + V] = base
+        check(padded[..., start:start + V], "padded, from %d" % start)
+        flat = torch.zeros(B * L * V + start, dtype=dtype, device=dev)
+        flat[start:] = base.reshape(-1)
+        check(flat[start:].view(B, L, V), "from element %d" % start)
+    check(base.transpose(0, 1).contiguous().transpose(0, 1), "time major")
+    check(base.permute(2, 0, 1).contiguous().permute(1, 2, 0), "word major")
+    check(base.view(B * L, V), "two dimensions", lambda t: t.reshape((B * L,) + t.shape[2:]))
+    check(base.view(B, 1, L, 1, V), "five dimensions", lambda t: t.reshape((B, 1, L, 1) + t.shape[2:]))
+    check(base[0, 0], "one row", lambda t: t[0, 0])
     # one row shown to all tokens: the gradient of the broadcast input is the sum over them
     one = base[:1, :1].detach().requires_grad_()
     wide = one.expand(B, L, V)
@@ -517,7 +520,7 @@ def test_gradients_against_differences(dev, kind):
 # ------------------------------------------------------------------------------------------------------------
 
 def test_more_logits_than_32_bits_count(dev):
-    """Rows behind the 2^31st element (and, in bytes, the 2^32nd) give the bits that they give alone."""
+    """Rows behind the 2^31st element (and, in bytes, the 2^32nd)."""
     from pevae_amd import ops
     T, V = 16500, 131072
     z = torch.empty(T, V, dtype=torch.bfloat16, device=dev)
@@ -527,25 +530,26 @@ def test_more_logits_than_32_bits_count(dev):
     y = torch.full((T,), -7, dtype=torch.int64, device=dev)
     y[-3:] = torch.tensor([0, V - 1, 4242], device=dev)
     z.requires_grad_()
-    small = tail.clone().requires_grad_()
-    a, b = ops.token_logprobs(z, y, ignore_index=-7), ops.token_logprobs(small, y[-3:], ignore_index=-7)
-    assert torch.equal(a[-3:], b) and float(a[:-3].abs().max()) == 0.0
-    g = torch.ones(T, device=dev)
-    da, = torch.autograd.grad(a, z, g)
-    db, = torch.autograd.grad(b, small, g[-3:])
-    assert torch.equal(da[-3:], db) and int(torch.count_nonzero(da[:-3])) == 0
-    del da
-    ids = tail.float().topk(4, -1)
-    all_ids = torch.zeros(T, 4, dtype=torch.int64, device=dev)
-    all_ids[-3:] = ids.indices
-    all_t = torch.zeros(T, 4, device=dev)
-    all_t[-3:] = ids.values
-    la = ops.distill_topk(z, all_ids, all_t, y, -7, avg_type=None)
-    lb = ops.distill_topk(small, ids.indices, ids.values, y[-3:], -7, avg_type=None)
-    assert abs(float(la - lb)) <= 2e-7 * abs(float(lb))
-    da, = torch.autograd.grad(la, z)
-    db, = torch.autograd.grad(lb, small)
-    assert torch.equal(da[-3:], db) and int(torch.count_nonzero(da[:-3])) == 0
+    p, lq = softmax64(tail, 1.0)
+    H = -plogp(p, lq).sum(-1)
+    one, none = torch.ones(3, dtype=torch.float64, device=dev), torch.zeros(3, dtype=torch.float64, device=dev)
+    lp = ops.token_logprobs(z, y, ignore_index=-7)
+    want = lq.gather(1, y[-3:, None])[:, 0]
+    close(lp[-3:], want, 1 + want.abs(), "logp")
+    assert float(lp[:-3].abs().max()) == 0.0
+    d, = torch.autograd.grad(lp, z, torch.ones(T, device=dev))
+    close(d[-3:], *rows_grad64(p, lq, H, y[-3:], one, none, 1.0), "dlogits")
+    assert int(torch.count_nonzero(d[:-3])) == 0
+    del d
+    top = tail.float().topk(4, -1)
+    ids, t = torch.zeros(T, 4, dtype=torch.int64, device=dev), torch.zeros(T, 4, device=dev)
+    ids[-3:], t[-3:] = top.indices, top.values
+    loss = ops.distill_topk(z, ids, t, y, -7, avg_type=None)
+    want, mag, dwant, dmag = distill64(tail, top.indices, top.values, one > 0, 1.0, 1.0)
+    close(loss, want, mag, "loss")
+    d, = torch.autograd.grad(loss, z)
+    close(d[-3:], dwant, dmag, "dlogits")
+    assert int(torch.count_nonzero(d[:-3])) == 0
 
 
 def test_many_rows(dev):
