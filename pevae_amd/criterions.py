@@ -175,6 +175,10 @@ class PreferenceLoss(_Loss):
         self.weight, self.avg_type = weight, avg_type
 
     def forward(self, chosen_output, chosen_labels, rejected_output, rejected_labels, ref_chosen=None, ref_rejected=None):
+        if not isinstance(chosen_output, DeferredLogProbs) and not isinstance(rejected_output, DeferredLogProbs):
+            return ops.vocab_preference_loss(chosen_output, chosen_labels, rejected_output, rejected_labels, ref_chosen,
+                                             ref_rejected, self.padding_idx, 1.0, self.beta, self.label_smoothing, self.weight,
+                                             self.avg_type)
         return ops.preference_loss(token_log_probs(chosen_output, chosen_labels, self.padding_idx), chosen_labels,
                                    token_log_probs(rejected_output, rejected_labels, self.padding_idx), rejected_labels,
                                    ref_chosen, ref_rejected, self.padding_idx, self.beta, self.label_smoothing, self.weight,

@@ -576,8 +576,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
 // ---- gradient: dz_v = g (e_v (a + b x_v) + d [v in the row's list]), pieces of rows dealt out to workgroups ----------------
 struct Grad {
   const float4* save;
-  const float *dlogp, *dent; // HEAD_TOKEN: upstream gradients a row
-  const float* g;            // else: upstream gradient of the loss (device scalar)
+  const float *dlogp, *dent; // HEAD_TOKEN: upstream gradients a row,
+  const float* slope;        // or, where not NULL, slope of the row's sequence times scale * *g
+  float scale;
+  const float* g;            // upstream gradient of the loss (device scalar)
   void* out;                 // [T][V]
   int ready;                 // out holds the gradient for *g = 1 already
 };
@@ -604,7 +606,7 @@ template <class E, int HEAD, int NT>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT, 8) void rows_grad_kernel(Rows a, Distill hd, Grad q, int blocks, long items) {
   typedef Place<NT> P;
   const int tid = P::tid();
-  const float up = HEAD == HEAD_TOKEN ? 1.f : *q.g;
+  const float up = q.g ? *q.g : 1.f;
   if (HEAD != HEAD_TOKEN && q.ready && up == 1.f) return;
   for (long it = P::row(); it < items; it += gridDim.x * (long)P::R) {
     const uint32_t t = (uint32_t)it / (uint32_t)blocks, share = (uint32_t)it - t * (uint32_t)blocks;   // items < 2^32
@@ -617,7 +619,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, 8) void rows_grad_kernel(Rows 
     float dy = 0.f;
     int y = -1;
     if (HEAD == HEAD_TOKEN) {
-      const float g = q.dlogp ? q.dlogp[t] : 0.f, h = q.dent ? q.dent[t] : 0.f, ln2 = 0.69314718056f;
+      const float g = q.slope ? up * q.scale * q.slope[sequence_of(a, t)] : q.dlogp ? q.dlogp[t] : 0.f;
+      const float h = q.dent ? q.dent[t] : 0.f, ln2 = 0.69314718056f;
       if (w.x != kDead) {
         w = make_float4(w.x, -a.c * w.y * (g - h * ln2 * w.z), -a.c * w.y * h * ln2, 0.f);
         dy = a.c * g;
@@ -771,22 +774,41 @@ __global__ __launch_bounds__(256) void add_counts_kernel(const float* __restrict
 }
 
 // ---- policy loss from log-probabilities ------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void policy_tokens_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels,
-                                                            int64_t ignore, long T, int n1, Policy h, float* __restrict__ dlp,
-                                                            Sum5* __restrict__ part, Result r) {
+// Latency bound: a few bytes a token.  One launch up to 4096 tokens, and one more that adds the workgroups' sums beyond.
+__global__ __launch_bounds__(1024) void policy_tokens_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels,
+                                                             int64_t ignore, long T, int n1, Policy h, float* __restrict__ dlp,
+                                                             Sum5* __restrict__ part, Result r) {
   __shared__ double sh[16][5];
   double v[5] = {0, 0, 0, 0, 0};
-  for (long t = blockIdx.x * 256L + threadIdx.x; t < T; t += gridDim.x * 256L) {
-    float d = 0.f;
-    if (labels[t] != ignore) {
-      const PolicyTerm q = policy_term(h, logp[t], h.old_lp[t], h.ref_lp ? h.ref_lp[t] : 0.f, h.adv[h.adv_per_row ? t : t / n1]);
-      v[0] += q.pg;
-      v[1] += q.k3;
-      v[2] += q.cut;
-      v[4] += 1.0;
-      d = q.dlp;
+  const long step = gridDim.x * 1024L;
+  for (long t0 = blockIdx.x * 1024L + threadIdx.x; t0 < T; t0 += 4 * step) {
+    float lp[4], old[4], ref[4], adv[4];
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                  // four tokens in flight; a dead one's entries may hold anything
+      const long t = t0 + i * step;
+      if (t >= T) break;
+      live[i] = labels[t] != ignore;
+      lp[i] = logp[t];
+      old[i] = h.old_lp[t];
+      ref[i] = h.ref_lp ? h.ref_lp[t] : 0.f;
+      adv[i] = h.adv[h.adv_per_row ? t : (long)((uint32_t)t / (uint32_t)n1)];
     }
-    if (dlp) dlp[t] = d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long t = t0 + i * step;
+      if (t >= T) break;
+      float d = 0.f;
+      if (live[i]) {
+        const PolicyTerm q = policy_term(h, lp[i], old[i], ref[i], adv[i]);
+        v[0] += q.pg;
+        v[1] += q.k3;
+        v[2] += q.cut;
+        v[4] += 1.0;
+        d = q.dlp;
+      }
+      if (dlp) dlp[t] = d;
+    }
   }
   block_sum(v, sh);
   if (threadIdx.x == 0) {
@@ -813,9 +835,20 @@ struct Answers {
 // sum over the live tokens of (log p - log p_ref), in fp64: long answers cancel
 __device__ __forceinline__ double answer_sum(const Answers& a, int64_t ignore, long b) {
   double v = 0.0;
-  for (int i = threadIdx.x; i < a.L; i += 256) {
-    const long t = b * a.L + i;
-    if (a.labels[t] != ignore) v += (double)a.logp[t] - (a.ref ? (double)a.ref[t] : 0.0);
+  for (int i0 = threadIdx.x; i0 < a.L; i0 += 4 * 256) {
+    int64_t y[4];
+    float lp[4], ref[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {                  // four tokens in flight; a dead one's entries may hold anything
+      const long t = b * a.L + i0 + k * 256;
+      const bool in = i0 + k * 256 < a.L;
+      y[k] = in ? a.labels[t] : ignore;
+      lp[k] = in ? a.logp[t] : 0.f;
+      ref[k] = in && a.ref ? a.ref[t] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (y[k] != ignore) v += (double)lp[k] - (double)ref[k];
   }
   return v;
 }
@@ -846,19 +879,15 @@ __global__ __launch_bounds__(256) void preference_kernel(Answers c, Answers r, i
   rowout[b] = make_float4(x != x ? x : loss, 0.f, 0.f, 0.f);
   slope[b] = beta * (smooth * sig - (1.f - smooth) * gis);
 }
-// d logp of both answers: +- g * scale * slope on live tokens
+// d logp of both answers of a pair: +- g * scale * slope on live tokens
 __global__ __launch_bounds__(256) void preference_bwd_kernel(const int64_t* __restrict__ labels_c, int Lc, float* __restrict__ dc,
                                                              const int64_t* __restrict__ labels_r, int Lr, float* __restrict__ dr,
-                                                             int64_t ignore, long P, const float* __restrict__ slope, float scale,
+                                                             int64_t ignore, const float* __restrict__ slope, float scale,
                                                              const float* __restrict__ g) {
-  const float w = *g * scale;
-  const long nc = P * Lc, n = nc + P * Lr;
-  for (long t = blockIdx.x * 256L + threadIdx.x; t < n; t += gridDim.x * 256L) {
-    if (t < nc)
-      dc[t] = labels_c[t] != ignore ? w * slope[t / Lc] : 0.f;
-    else
-      dr[t - nc] = labels_r[t - nc] != ignore ? -w * slope[(t - nc) / Lr] : 0.f;
-  }
+  const long b = blockIdx.x;
+  const float w = *g * scale * slope[b];
+  for (int i = threadIdx.x; i < Lc; i += 256) dc[b * Lc + i] = labels_c[b * Lc + i] != ignore ? w : 0.f;
+  for (int i = threadIdx.x; i < Lr; i += 256) dr[b * Lr + i] = labels_r[b * Lr + i] != ignore ? -w : 0.f;
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
@@ -874,21 +903,33 @@ int check_rows(const char* who, const void* logits, int dtype, long n0, int n1, 
   }
   return PV_OK;
 }
+int check_count(const char* who, long n) {
+  if (n <= 0x7fffffffL) return PV_OK;
+  pv_set_error("%s: %ld are beyond the limit of 2^31 - 1", who, n);
+  return PV_ERR_LIMIT;
+}
 Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, const int64_t* labels, int64_t ignore, float c) {
   return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore};
 }
 
 inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
 
+// Threads a row of the pass that only reads: a wave for short rows (V = 5003, bf16, 20000 rows: 39 us, 256 threads 49), more
+// for longer ones (V = 20004, bf16, 12800 rows, half of them dead: 256 threads 49 us, 64 58, 1024 82; V = 64001, fp32, 3000 rows:
+// 1024 threads 125 us, 256 132; one row of V = 131071, fp32: 1024 threads 10.4 us, 256 17.5).  Splitting one row over workgroups
+// and joining the parts in a second launch took 9.4 us there, and more than one launch everywhere else.
 template <class E, int HEAD, bool ENT>
 int launch_fwd_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
   const int pieces = a.V / E::N;
-  if (pieces <= 512)
-    rows_fwd_kernel<E, HEAD, ENT, 64><<<dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st>>>(a, hp, hd, sc, o);
-  else if (pieces <= 2048 || a.T >= 512)
-    rows_fwd_kernel<E, HEAD, ENT, 256><<<dim3((unsigned)a.T), dim3(256), 0, st>>>(a, hp, hd, sc, o);
-  else                                             // few long rows: a whole CU for each
-    rows_fwd_kernel<E, HEAD, ENT, 1024><<<dim3((unsigned)a.T), dim3(1024), 0, st>>>(a, hp, hd, sc, o);
+  const unsigned T = (unsigned)a.T;
+  if (pieces <= 256 || (pieces <= 1024 && T >= 512))
+    rows_fwd_kernel<E, HEAD, ENT, 64><<<dim3((T + 3) / 4), dim3(256), 0, st>>>(a, hp, hd, sc, o);
+  else if (pieces <= 4096)
+    rows_fwd_kernel<E, HEAD, ENT, 256><<<dim3(T), dim3(256), 0, st>>>(a, hp, hd, sc, o);
+  else if (pieces <= 6144 && T >= 512)
+    rows_fwd_kernel<E, HEAD, ENT, 512><<<dim3(T), dim3(512), 0, st>>>(a, hp, hd, sc, o);
+  else
+    rows_fwd_kernel<E, HEAD, ENT, 1024><<<dim3(T), dim3(1024), 0, st>>>(a, hp, hd, sc, o);
   PV_LAUNCH_CHECK("rows_fwd_kernel");
   return PV_OK;
 }
@@ -1018,7 +1059,7 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && save && dlogits && (dlogp || dentropy), "pv_token_logp_bwd: null argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
-  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, dlogp, dentropy, nullptr, dlogits, 0},
+  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, dlogp, dentropy, nullptr, 0.f, nullptr, dlogits, 0},
                                  (hipStream_t)stream);
 }
 
@@ -1056,7 +1097,7 @@ int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, 
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && save && g && dlogits, "pv_policy_rows_bwd: null argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
-  return launch_grad<HEAD_POLICY>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, g, dlogits, ready},
+  return launch_grad<HEAD_POLICY>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, nullptr, 0.f, g, dlogits, ready},
                                   (hipStream_t)stream);
 }
 
@@ -1104,7 +1145,7 @@ int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0,
   PV_REQUIRE(t_ids && save && psum && g && dlogits && K > 0 && K <= kTeacherMax, "pv_distill_rows_bwd: bad argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, nullptr, 0, inv_temp);
   return launch_grad<HEAD_DISTILL>(dtype, a, Distill{t_ids, nullptr, K, 0, (float*)psum},
-                                   Grad{(const float4*)save, nullptr, nullptr, g, dlogits, ready}, (hipStream_t)stream);
+                                   Grad{(const float4*)save, nullptr, nullptr, nullptr, 0.f, g, dlogits, ready}, (hipStream_t)stream);
 }
 
 int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,
@@ -1114,11 +1155,12 @@ int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignor
   PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_tokens_fwd: the clip range is empty");
   hipStream_t st = (hipStream_t)stream;
   const long T = n0 * (long)n1;
+  if (check_count("pv_policy_tokens_fwd", T) != PV_OK) return PV_ERR_LIMIT;
   const Policy h = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, 0.f};
   const Result r = {kl_coef, 0.f, weight, word, loss, stats, dlogp ? dlogp + T : nullptr};
-  const long want = (T + 255) / 256;
+  const long want = T <= 4096 ? 1 : (T + 1023) / 1024;
   const int g = (int)(want > kSumGroups ? kSumGroups : want);
-  policy_tokens_kernel<<<dim3(g), dim3(256), 0, st>>>(logp, tokens, ignore, T, n1, h, dlogp, (Sum5*)ws, r);
+  policy_tokens_kernel<<<dim3(g), dim3(1024), 0, st>>>(logp, tokens, ignore, T, n1, h, dlogp, (Sum5*)ws, r);
   PV_LAUNCH_CHECK("policy_tokens_kernel");
   if (g > 1) {
     sum_parts_kernel<<<dim3(1), dim3(256), 0, st>>>((const Sum5*)ws, g, r);
@@ -1141,10 +1183,7 @@ int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* la
                       float smoothing, float weight, float* loss, float* rewards, float* slope, void* ws, void* stream) {
   PV_REQUIRE(loss && rewards && slope && ws && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_fwd: bad argument");
   PV_REQUIRE((Lc == 0 || (logp_c && labels_c)) && (Lr == 0 || (logp_r && labels_r)), "pv_preference_fwd: null argument");
-  if (pairs > 0x7fffffffL) {
-    pv_set_error("pv_preference_fwd: %ld pairs are beyond the limit of 2^31 - 1", pairs);
-    return PV_ERR_LIMIT;
-  }
+  if (check_count("pv_preference_fwd", pairs) != PV_OK) return PV_ERR_LIMIT;
   hipStream_t st = (hipStream_t)stream;
   float4* rowout = (float4*)ws;
   preference_kernel<<<dim3((unsigned)pairs), dim3(256), 0, st>>>(Answers{logp_c, ref_c, labels_c, Lc},
@@ -1154,14 +1193,43 @@ int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* la
   return launch_sum(rowout, nullptr, 0, pairs, (Sum5*)(rowout + pairs), Result{0.f, 0.f, weight, 0, loss, nullptr, nullptr}, st);
 }
 
+int pv_preference_rows_fwd(const void* logits_c, int dtype_c, long pairs, int Lc, long s0c, long s1c, int Vc,
+                           const int64_t* labels_c, const float* ref_c, const void* logits_r, int dtype_r, int Lr, long s0r,
+                           long s1r, int Vr, const int64_t* labels_r, const float* ref_r, int64_t ignore, float inv_temp,
+                           float beta, float smoothing, float weight, float* loss, float* rewards, float* slope, float* save_c,
+                           float* save_r, void* ws, void* stream) {
+  int rc = check_rows("pv_preference_rows_fwd", logits_c, dtype_c, pairs, Lc, s0c, s1c, Vc, inv_temp);
+  if (rc == PV_OK) rc = check_rows("pv_preference_rows_fwd", logits_r, dtype_r, pairs, Lr, s0r, s1r, Vr, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(labels_c && labels_r && loss && rewards && slope && ws, "pv_preference_rows_fwd: null argument");
+  float* lp_c = (float*)((char*)ws + pv_vocab_rows_ws_bytes(pairs));
+  float* lp_r = lp_c + pairs * Lc;
+  rc = pv_token_logp_fwd(logits_c, dtype_c, pairs, Lc, s0c, s1c, Vc, labels_c, ignore, inv_temp, lp_c, nullptr, save_c, stream);
+  if (rc == PV_OK)
+    rc = pv_token_logp_fwd(logits_r, dtype_r, pairs, Lr, s0r, s1r, Vr, labels_r, ignore, inv_temp, lp_r, nullptr, save_r, stream);
+  if (rc != PV_OK) return rc;
+  return pv_preference_fwd(lp_c, ref_c, labels_c, Lc, lp_r, ref_r, labels_r, Lr, pairs, ignore, beta, smoothing, weight, loss,
+                           rewards, slope, ws, stream);
+}
+
+int pv_preference_rows_bwd(const void* logits, int dtype, long pairs, int L, long s0, long s1, int V, const int64_t* labels,
+                           int64_t ignore, float inv_temp, const float* save, const float* slope, float weight, const float* g,
+                           void* dlogits, void* stream) {
+  const int rc = check_rows("pv_preference_rows_bwd", logits, dtype, pairs, L, s0, s1, V, inv_temp);
+  if (rc != PV_OK) return rc;
+  PV_REQUIRE(labels && save && slope && g && dlogits, "pv_preference_rows_bwd: null argument");
+  const Rows a = make_rows(logits, pairs, L, s0, s1, V, labels, ignore, inv_temp);
+  return launch_grad<HEAD_TOKEN>(dtype, a, Distill{}, Grad{(const float4*)save, nullptr, nullptr, slope, weight, g, dlogits, 0},
+                                 (hipStream_t)stream);
+}
+
 int pv_preference_bwd(const int64_t* labels_c, int Lc, const int64_t* labels_r, int Lr, long pairs, int64_t ignore,
                       const float* slope, float weight, const float* g, float* dlogp_c, float* dlogp_r, void* stream) {
   PV_REQUIRE(slope && g && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_bwd: bad argument");
   PV_REQUIRE((Lc == 0 || (labels_c && dlogp_c)) && (Lr == 0 || (labels_r && dlogp_r)), "pv_preference_bwd: null argument");
-  const long n = pairs * ((long)Lc + Lr), want = (n + 255) / 256;
-  if (n == 0) return PV_OK;
-  preference_bwd_kernel<<<dim3((unsigned)(want > 2048 ? 2048 : want)), dim3(256), 0, (hipStream_t)stream>>>(
-      labels_c, Lc, dlogp_c, labels_r, Lr, dlogp_r, ignore, pairs, slope, weight, g);
+  if (check_count("pv_preference_bwd", pairs) != PV_OK) return PV_ERR_LIMIT;
+  preference_bwd_kernel<<<dim3((unsigned)pairs), dim3(256), 0, (hipStream_t)stream>>>(labels_c, Lc, dlogp_c, labels_r, Lr, dlogp_r,
+                                                                                      ignore, slope, weight, g);
   PV_LAUNCH_CHECK("preference_bwd_kernel");
   return PV_OK;
 }

@@ -4,6 +4,7 @@ PyTorch is used here for device memory, streams and autograd bookkeeping only: e
 is a hand-written HIP kernel from libpevae_hip.so, launched on torch's current stream.  Nothing in this file
 has a CPU path -- CPU tensors raise.
 """
+import builtins
 import ctypes as C
 
 import os
@@ -2768,6 +2769,31 @@ def _avg(avg_type, weight, sequences):
     raise ValueError("Unknown avg type")
 
 
+_WS_BASE = None
+
+
+def _ws_bytes(rows):
+    """pv_vocab_rows_ws_bytes(rows): a fixed part, and 16 bytes a row."""
+    global _WS_BASE
+    if _WS_BASE is None:
+        _WS_BASE = _lib.load().pv_vocab_rows_ws_bytes(0)
+    return _WS_BASE + 16 * rows
+
+
+def _align16(n):
+    return (n + 15) // 16 * 16
+
+
+def _pieces(dev, *sizes):
+    """One allocation for what a call keeps or scribbles on: (tensor, address of each piece, 16-byte aligned)."""
+    buf = torch.empty(builtins.sum(map(_align16, sizes)), dtype=torch.uint8, device=dev)
+    at, out = buf.data_ptr(), [buf]
+    for n in sizes:
+        out.append(at)
+        at += _align16(n)
+    return out
+
+
 def _one_pass_grad(logits, want):
     """The gradient's tensor where the forward pass writes it: rows that fit the kernel that holds them on chip."""
     if want and _lib.load().pv_vocab_rows_one_pass(_ROW_DTYPES[logits.dtype], logits.shape[-1]):
@@ -2840,26 +2866,24 @@ class DistillTopK(torch.autograd.Function):
         dev, K = x.device, ids.shape[-1]
         T = ids.numel() // K
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
-        psum = torch.empty((T, K), dtype=torch.float32, device=dev)
+        buf, save, psum, ws = _pieces(dev, 16 * T, 4 * T * K, _ws_bytes(T))
         d = _one_pass_grad(logits, want_grad)
-        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
         _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, _p(ids), _p(t_logits),
-                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), _p(save), _p(psum), _p(d), _p(ws))
+                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), save if want_grad else None, psum, _p(d), ws)
         if want_grad:
-            ctx.save_for_backward(x, ids, save, psum)
+            ctx.save_for_backward(x, ids, buf)
             ctx.grad = d
-        ctx.meta = (inv_temp, K, logits.shape)
+        ctx.meta = (inv_temp, K, T, logits.shape)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, ids, save, psum = ctx.saved_tensors
-        inv_temp, K, shape = ctx.meta
+        x, ids, buf = ctx.saved_tensors
+        inv_temp, K, T, shape = ctx.meta
         d, ready = _take_grad(ctx, x, shape)
-        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(save), _p(psum), _p(g.contiguous()), ready,
-                _p(d))
+        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(buf), _p(buf) + _align16(16 * T), _p(g),
+                ready, _p(d))
         return (d,) + (None,) * 8
 
 
@@ -2906,13 +2930,13 @@ class VocabPolicyLoss(torch.autograd.Function):
         x = _plain_rows(logits)
         dev, T = x.device, tokens.numel()
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
-        save = torch.empty((T, 4), dtype=torch.float32, device=dev) if want_grad else None
+        buf, save, ws = _pieces(dev, 16 * T, _ws_bytes(T))
         d = _one_pass_grad(logits, want_grad)
-        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(T), dtype=torch.uint8, device=dev)
         _launch(dev, "pv_policy_rows_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(old), _p(ref), _p(adv),
-                int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), _p(save), _p(d), _p(ws))
+                int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), save if want_grad else None,
+                _p(d), ws)
         if want_grad:
-            ctx.save_for_backward(x, tokens, save)
+            ctx.save_for_backward(x, tokens, buf)
             ctx.grad = d
         ctx.meta = (ignore, inv_temp, logits.shape)
         ctx.mark_non_differentiable(stats)
@@ -2921,11 +2945,10 @@ class VocabPolicyLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _dstats):
-        x, tokens, save = ctx.saved_tensors
+        x, tokens, buf = ctx.saved_tensors
         ignore, inv_temp, shape = ctx.meta
         d, ready = _take_grad(ctx, x, shape)
-        _launch(x.device, "pv_policy_rows_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(save), _p(g.contiguous()), ready,
-                _p(d))
+        _launch(x.device, "pv_policy_rows_bwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(buf), _p(g), ready, _p(d))
         return (d,) + (None,) * 13
 
 
@@ -2938,12 +2961,11 @@ class PolicyLoss(torch.autograd.Function):
         dev, T = x.device, tokens.numel()
         n1 = x.shape[1] if x.dim() == 2 else T
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
-        dlp = torch.empty(T + 1, dtype=torch.float32, device=dev) if want_grad else None
-        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(0), dtype=torch.uint8, device=dev)
+        buf, dlp, ws = _pieces(dev, 4 * (T + 1), _ws_bytes(0))
         _launch(dev, "pv_policy_tokens_fwd", _p(x), _p(tokens), ignore, T // n1, n1, _p(old), _p(ref), _p(adv),
-                int(adv.numel() == T), lo, hi, kl, weight, word, _p(loss), _p(stats), _p(dlp), _p(ws))
+                int(adv.numel() == T), lo, hi, kl, weight, word, _p(loss), _p(stats), dlp if want_grad else None, ws)
         if want_grad:
-            ctx.save_for_backward(dlp)
+            ctx.save_for_backward(buf)
         ctx.shape = logp.shape
         ctx.mark_non_differentiable(stats)
         return loss, stats
@@ -2951,9 +2973,9 @@ class PolicyLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _dstats):
-        dlp, = ctx.saved_tensors
-        d = torch.empty(ctx.shape, dtype=torch.float32, device=dlp.device)
-        _launch(dlp.device, "pv_policy_tokens_bwd", _p(dlp), _p(g.contiguous()), d.numel(), _p(d))
+        buf, = ctx.saved_tensors
+        d = torch.empty(ctx.shape, dtype=torch.float32, device=buf.device)
+        _launch(buf.device, "pv_policy_tokens_bwd", _p(buf), _p(g), d.numel(), _p(d))
         return (d,) + (None,) * 11
 
 
@@ -3021,11 +3043,10 @@ class PreferenceLoss(torch.autograd.Function):
         dev, P = xc.device, xc.shape[0]
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
-        slope = torch.empty(P, dtype=torch.float32, device=dev)
-        ws = torch.empty(_lib.load().pv_vocab_rows_ws_bytes(P), dtype=torch.uint8, device=dev)
+        buf, slope, ws = _pieces(dev, 4 * P, _ws_bytes(P))
         _launch(dev, "pv_preference_fwd", _p(xc), _p(ref_c), _p(labels_c), xc.shape[1], _p(xr), _p(ref_r), _p(labels_r),
-                xr.shape[1], P, ignore, beta, smoothing, weight, _p(loss), _p(rewards), _p(slope), _p(ws))
-        ctx.save_for_backward(labels_c, labels_r, slope)
+                xr.shape[1], P, ignore, beta, smoothing, weight, _p(loss), _p(rewards), slope, ws)
+        ctx.save_for_backward(labels_c, labels_r, buf)
         ctx.meta = (ignore, weight)
         rc, rr = rewards[0], rewards[1]
         ctx.mark_non_differentiable(rc, rr)
@@ -3034,13 +3055,90 @@ class PreferenceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _drc, _drr):
-        labels_c, labels_r, slope = ctx.saved_tensors
+        labels_c, labels_r, buf = ctx.saved_tensors
         ignore, weight = ctx.meta
-        dc = torch.empty(labels_c.shape, dtype=torch.float32, device=slope.device)
-        dr = torch.empty(labels_r.shape, dtype=torch.float32, device=slope.device)
-        _launch(slope.device, "pv_preference_bwd", _p(labels_c), labels_c.shape[1], _p(labels_r), labels_r.shape[1],
-                slope.numel(), ignore, _p(slope), weight, _p(g.contiguous()), _p(dc), _p(dr))
+        dc = torch.empty(labels_c.shape, dtype=torch.float32, device=buf.device)
+        dr = torch.empty(labels_r.shape, dtype=torch.float32, device=buf.device)
+        _launch(buf.device, "pv_preference_bwd", _p(labels_c), labels_c.shape[1], _p(labels_r), labels_r.shape[1],
+                labels_c.shape[0], ignore, _p(buf), weight, _p(g), _p(dc), _p(dr))
         return (dc, dr) + (None,) * 8
+
+
+class VocabPreferenceLoss(torch.autograd.Function):
+    """The preference loss of pairs of answers from the logits of their rows."""
+
+    @staticmethod
+    def forward(ctx, logits_c, logits_r, labels_c, labels_r, ref_c, ref_r, ignore, inv_temp, beta, smoothing, weight, grad_c, grad_r):
+        xc, xr = _plain_rows(logits_c), _plain_rows(logits_r)
+        dev, P, Tc, Tr = xc.device, xc.shape[0], labels_c.numel(), labels_r.numel()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
+        buf, slope, save_c, save_r, ws = _pieces(dev, 4 * P, 16 * Tc, 16 * Tr, _ws_bytes(P) + 4 * (Tc + Tr))
+        ac, ar = _row_args(xc), _row_args(xr)
+        _launch(dev, "pv_preference_rows_fwd", *ac, _p(labels_c), _p(ref_c), *ar[:2], *ar[3:], _p(labels_r), _p(ref_r), ignore,
+                inv_temp, beta, smoothing, weight, _p(loss), _p(rewards), slope, save_c if grad_c else None,
+                save_r if grad_r else None, ws)
+        if grad_c or grad_r:
+            ctx.save_for_backward(xc if grad_c else None, xr if grad_r else None, labels_c, labels_r, buf)
+        ctx.meta = (ignore, inv_temp, weight)
+        rc, rr = rewards[0], rewards[1]
+        ctx.mark_non_differentiable(rc, rr)
+        return loss, rc, rr
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _drc, _drr):
+        xc, xr, labels_c, labels_r, buf = ctx.saved_tensors
+        ignore, inv_temp, weight = ctx.meta
+        slope = _p(buf)
+        save = slope + _align16(4 * labels_c.shape[0])
+        out = []
+        for x, labels, w in ((xc, labels_c, weight), (xr, labels_r, -weight)):
+            d = None
+            if x is not None:
+                d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                _launch(x.device, "pv_preference_rows_bwd", *_row_args(x), _p(labels), ignore, inv_temp, save, slope, w, _p(g), _p(d))
+            out.append(d)
+            save += 16 * labels.numel()            # (the chosen answer's rows lie before the rejected one's)
+        return tuple(out) + (None,) * 11
+
+
+def _preference_args(shape_c, shape_r, chosen_labels, rejected_labels, ref_chosen, ref_rejected, label_smoothing, avg_type):
+    if shape_c[0] != shape_r[0]:
+        raise ValueError("%d chosen and %d rejected answers" % (shape_c[0], shape_r[0]))
+    if (ref_chosen is None) != (ref_rejected is None):
+        raise ValueError("a reference model's log-probabilities are needed for both answers, or for neither")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("label_smoothing must lie in [0, 1] (got %r)" % (label_smoothing,))
+    if avg_type not in ("seq", None):
+        raise ValueError("Unknown avg type")
+    return (_index("chosen_labels", chosen_labels, shape_c), _index("rejected_labels", rejected_labels, shape_r),
+            _constant("ref_chosen", ref_chosen, shape_c), _constant("ref_rejected", ref_rejected, shape_r))
+
+
+def vocab_preference_loss(chosen_logits, chosen_labels, rejected_logits, rejected_labels, ref_chosen=None, ref_rejected=None,
+                          ignore_index=None, inv_temp=1.0, beta=0.1, label_smoothing=0.0, weight=1.0, avg_type="seq"):
+    """preference_loss from the logits [P, Lc, V] / [P, Lr, V] of both answers' rows (at the inverse temperature `inv_temp`):
+    their log-probabilities, the loss and both gradients without anything else of the logits' size.
+    -> (loss, chosen rewards [P], rejected rewards [P]); the loss is differentiable in both logits."""
+    for x in (chosen_logits, rejected_logits):
+        _check_rows(x)
+        if x.dim() != 3:
+            raise ValueError("logits must be [P, L, V] (got shape %s)" % (tuple(x.shape),))
+    _check_temp(inv_temp)
+    shape_c, shape_r = tuple(chosen_logits.shape[:2]), tuple(rejected_logits.shape[:2])
+    lc, lr, rc, rr = _preference_args(shape_c, shape_r, chosen_labels, rejected_labels, ref_chosen, ref_rejected, label_smoothing,
+                                      avg_type)
+    _same_device(chosen_logits, chosen_labels, rejected_logits, rejected_labels, ref_chosen, ref_rejected)
+    if lc.numel() == 0 or lr.numel() == 0:         # an answer without rows: through the log-probabilities
+        return preference_loss(token_logprobs(chosen_logits, lc, ignore_index, inv_temp), lc,
+                               token_logprobs(rejected_logits, lr, ignore_index, inv_temp), lr, rc, rr, ignore_index, beta,
+                               label_smoothing, weight, avg_type)
+    on = torch.is_grad_enabled()
+    return VocabPreferenceLoss.apply(chosen_logits, rejected_logits, lc, lr, rc, rr,
+                                     _NO_INDEX if ignore_index is None else int(ignore_index), float(inv_temp), float(beta),
+                                     float(label_smoothing), _avg(avg_type, weight, shape_c[0])[0],
+                                     on and chosen_logits.requires_grad, on and rejected_logits.requires_grad)
 
 
 def preference_loss(chosen_logp, chosen_labels, rejected_logp, rejected_labels, ref_chosen=None, ref_rejected=None,
@@ -3053,17 +3151,8 @@ def preference_loss(chosen_logp, chosen_labels, rejected_logp, rejected_labels, 
     for name, t in (("chosen_logp", chosen_logp), ("rejected_logp", rejected_logp)):
         if t.dim() != 2 or t.dtype != torch.float32:
             raise ValueError("%s must be float32 [P, L] (got %s %s)" % (name, t.dtype, tuple(t.shape)))
-    if chosen_logp.shape[0] != rejected_logp.shape[0]:
-        raise ValueError("%d chosen and %d rejected answers" % (chosen_logp.shape[0], rejected_logp.shape[0]))
-    if (ref_chosen is None) != (ref_rejected is None):
-        raise ValueError("a reference model's log-probabilities are needed for both answers, or for neither")
-    if not 0.0 <= label_smoothing <= 1.0:
-        raise ValueError("label_smoothing must lie in [0, 1] (got %r)" % (label_smoothing,))
-    if avg_type not in ("seq", None):
-        raise ValueError("Unknown avg type")
-    lc = _index("chosen_labels", chosen_labels, chosen_logp.shape)
-    lr = _index("rejected_labels", rejected_labels, rejected_logp.shape)
-    rc, rr = _constant("ref_chosen", ref_chosen, chosen_logp.shape), _constant("ref_rejected", ref_rejected, rejected_logp.shape)
+    lc, lr, rc, rr = _preference_args(tuple(chosen_logp.shape), tuple(rejected_logp.shape), chosen_labels, rejected_labels,
+                                      ref_chosen, ref_rejected, label_smoothing, avg_type)
     _same_device(chosen_logp, chosen_labels, rejected_logp, rejected_labels, ref_chosen, ref_rejected)
     P = chosen_logp.shape[0]
     if P == 0:

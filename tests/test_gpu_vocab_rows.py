@@ -462,6 +462,53 @@ def test_preference_loss(dev, P, Lc, Lr, smooth, with_ref, avg):
     close(dr, 3 * slope[:, None] * (yr != -7), 3 * mag[:, None] * (yr != -7), "rejected gradient")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("P,Lc,Lr,V", [(1, 1, 1, 7), (3, 4, 2, 1009), (2, 3, 5, 20003), (5, 2, 3, 260), (2, 0, 3, 50)])
+@pytest.mark.parametrize("smooth,with_ref,avg", [(0.0, True, "seq"), (0.2, False, None)])
+def test_vocab_preference_loss(dev, dtype, P, Lc, Lr, V, smooth, with_ref, avg):
+    """From the logits: the log-probabilities' errors (5e-6 a token, see above) add up in the rewards."""
+    from pevae_amd import ops
+    beta, c = 0.25, 1.0 / 0.9
+    side = []
+    for L, seed in ((Lc, 150), (Lr, 160)):
+        z = make((P, L, V), dtype, dev, seed).requires_grad_()
+        y = labels_of((P, L), V, dev, seed + 1)
+        live = y != -7
+        p, lq = softmax64(z, c) if L else (z.detach().double(), z.detach().double())
+        lp = lq.gather(-1, y.clamp(min=0)[..., None])[..., 0]
+        ref = (lp.float() + 0.3 * make((P, L), torch.float32, dev, seed + 2, 1.0)) if with_ref else None
+        d = torch.where(live, lp - (0 if ref is None else ref.double()), torch.zeros_like(lp))
+        rmag = (live * (1 + lp.abs() + (0 if ref is None else ref.double().abs()))).sum(1)
+        if ref is not None:
+            ref = torch.where(live, ref, torch.full_like(ref, float("nan")))
+        side.append((z, y, live, p, lq, ref, beta * d.sum(1), beta * rmag))
+    (zc, yc, livec, pc, lqc, refc, rwc, mc), (zr, yr, liver, pr, lqr, refr, rwr, mr) = side
+    loss, got_c, got_r = ops.vocab_preference_loss(zc, yc, zr, yr, refc, refr, -7, c, beta, smooth, 3.0, avg)
+    close(got_c, rwc, mc + 1e-30, "chosen")
+    close(got_r, rwr, mr + 1e-30, "rejected")
+    x, xmag = rwc - rwr, mc + mr
+    n = P if avg == "seq" else 1
+    rows = -(1 - smooth) * torch.nn.functional.logsigmoid(x) - smooth * torch.nn.functional.logsigmoid(-x)
+    close(loss, 3.0 / n * rows.sum(), 3.0 / n * (rows.abs() + xmag + 0.1).sum(), "loss")
+    slope = 3.0 / n * beta * (smooth * torch.sigmoid(x) - (1 - smooth) * torch.sigmoid(-x))
+    smag = 3.0 / n * beta * (1 + xmag)
+    zero = {True: torch.zeros(P, Lc, dtype=torch.float64, device=dev), False: torch.zeros(P, Lr, dtype=torch.float64, device=dev)}
+    for up in (None, torch.tensor(-2.0, device=dev)):
+        k = 1.0 if up is None else -2.0
+        dc, dr = torch.autograd.grad(loss, [zc, zr], up, retain_graph=True)
+        for d, z, y, live, p, lq, sign, side_ in ((dc, zc, yc, livec, pc, lqc, 1, True), (dr, zr, yr, liver, pr, lqr, -1, False)):
+            yl = torch.where(live, y, torch.full_like(y, -1))
+            h = zero[side_]
+            if not y.numel():
+                assert d.shape == z.shape
+                continue
+            want, _ = rows_grad64(p, lq, h, yl, k * sign * slope[:, None] * live, h, c)
+            _, mag = rows_grad64(p, lq, h, yl, abs(k) * smag[:, None] * live, h, c)
+            close(d, want, mag, "gradient")
+    only, = torch.autograd.grad(ops.vocab_preference_loss(zc.detach(), yc, zr, yr, refc, refr, -7, c, beta, smooth, 3.0, avg)[0], zr)
+    assert torch.equal(only, torch.autograd.grad(loss, zr)[0])
+
+
 def test_preference_far_apart(dev):
     """Rewards far apart: the loss is 0 or the distance, without overflow; infinite ones stay infinite."""
     from pevae_amd import ops
@@ -577,7 +624,7 @@ def test_empty_batches(dev):
     lp = ops.token_logprobs(z, y)
     assert lp.shape == (0, 4)
     for loss in (ops.distill_topk(z, y[..., None], f[..., None]), ops.vocab_policy_loss(z, y, f, f)[0],
-                 ops.policy_loss(lp, y, f, f)[0], ops.preference_loss(lp, y, lp, y)[0]):
+                 ops.policy_loss(lp, y, f, f)[0], ops.preference_loss(lp, y, lp, y)[0], ops.vocab_preference_loss(z, y, z, y)[0]):
         assert float(loss) == 0.0
         assert torch.autograd.grad(loss, z, retain_graph=True)[0].shape == z.shape
 
@@ -596,8 +643,9 @@ def test_same_bits_every_time_and_on_another_stream(dev):
         a = ops.distill_topk(z, t.indices, t.values, y, -7, avg_type="word")
         b, stats = ops.vocab_policy_loss(z, y, old, adv, old + 0.1, -7, kl_coef=0.1, ent_coef=0.01)
         c, rc, rr = ops.preference_loss(lp[:20], y[:20], lp[20:], y[20:], ignore_index=-7)
-        ga, gb, gc = (torch.autograd.grad(x, z, retain_graph=True)[0] for x in (a, b, c))
-        return [x.detach() for x in (lp, H, a, b, stats, c, rc, rr, ga, gb, gc)]
+        e = ops.vocab_preference_loss(z[:20], y[:20], z[20:], y[20:], ignore_index=-7)[0]
+        grads = [torch.autograd.grad(x, z, retain_graph=True)[0] for x in (a, b, c, e)]
+        return [x.detach() for x in (lp, H, a, b, stats, c, rc, rr, e)] + grads
 
     first = once()
     torch.cuda.synchronize()
@@ -629,9 +677,10 @@ def test_captured_and_replayed(dev):
         b, stats = ops.vocab_policy_loss(z, y, old, adv, old, -7, kl_coef=0.1)
         c = ops.preference_loss(lp[:B], y[:B], lp[B:], y[B:], old[:B], old[B:], -7)[0]
         e = ops.policy_loss(lp, y, old, adv, ignore_index=-7)[0]
-        grads = [torch.autograd.grad(x, z, retain_graph=True)[0] for x in (a, b, c, e)]
+        f = ops.vocab_preference_loss(z[:B], y[:B], z[B:], y[B:], old[:B], old[B:], -7)[0]
+        grads = [torch.autograd.grad(x, z, retain_graph=True)[0] for x in (a, b, c, e, f)]
         half = torch.autograd.grad(a, z, torch.full_like(a, 0.5), retain_graph=True)[0]
-        return [x.detach() for x in (lp, a, b, stats, c, e)] + grads + [half]
+        return [x.detach() for x in (lp, a, b, stats, c, e, f)] + grads + [half]
 
     inputs = [make((2 * B, L, V), torch.bfloat16, dev, s) for s in (93, 94)]
     held = [x.clone().requires_grad_() for x in inputs]

@@ -25,7 +25,8 @@ def test_valid_arguments_on_the_cpu_raise_for_the_device():
                  lambda: ops.distill_topk(rows(), ids(2, 3, 2), f(2, 3, 2), ids(2, 3), 0),
                  lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(2)),
                  lambda: ops.policy_loss(f(2, 3), ids(2, 3), f(2, 3), f(2, 3)),
-                 lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 4), ids(2, 4))):
+                 lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 4), ids(2, 4)),
+                 lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(L=4), ids(2, 4))):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
 
@@ -58,6 +59,10 @@ def test_valid_arguments_on_the_cpu_raise_for_the_device():
     lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), ref_chosen=f(2, 3)),
     lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), label_smoothing=1.5),
     lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 3), ids(2, 3), avg_type="word"),
+    lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(B=3), ids(3, 3)),
+    lambda: ops.vocab_preference_loss(rows()[0], ids(3), rows()[0], ids(3)),
+    lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(), ids(2, 3), f(2, 3)),
+    lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(), ids(2, 3), f(2, 3).requires_grad_(), f(2, 3)),
 ])
 def test_bad_arguments_raise_value_errors(call):
     with pytest.raises(ValueError):
@@ -92,5 +97,8 @@ def test_entry_points_refuse_on_the_host():
     assert lib.pv_vocab_rows_one_pass(0, 81923) == 1 and lib.pv_vocab_rows_one_pass(0, 81924) == 0     # 20 480 pieces of 16 bytes
     assert lib.pv_vocab_rows_one_pass(1, 163847) == 1 and lib.pv_vocab_rows_one_pass(2, 163848) == 0
     assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 81924, 81924, None, 0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, p, None) == -1
+    assert lib.pv_preference_rows_fwd(p, 0, 2, 3, 15, 5, 5, p, None, p, 0, 0, 15, 5, 5, p, None, 0, 1.0, 0.1, 0.0, 1.0, p, p, p, p, p, p,
+                                      None) == -1
+    assert lib.pv_preference_rows_bwd(p, 0, 2, 3, 15, 5, 5, p, 0, 1.0, None, p, 1.0, p, p, None) == -1
     assert lib.pv_distill_max_entries() == 256
     assert lib.pv_vocab_rows_ws_bytes(10) >= 160
