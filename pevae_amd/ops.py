@@ -4,7 +4,6 @@ PyTorch is used here for device memory, streams and autograd bookkeeping only: e
 is a hand-written HIP kernel from libpevae_hip.so, launched on torch's current stream.  Nothing in this file
 has a CPU path -- CPU tensors raise.
 """
-import builtins
 import ctypes as C
 
 import os
@@ -2689,18 +2688,31 @@ _NO_INDEX = -(1 << 63)           # an ignore index that no label has
 def _launch(dev, name, *args):
     """One C call on `dev`'s current stream, whatever the current device is.  (The raw handle: the Stream object around it
     costs more than the launch of a small kernel.)"""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
+    at = dev.index
+    if at != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+            return _launch(dev, name, *args)
+    rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _same_device(*ts):
-    _need_cuda(*ts)
-    dev = ts[0].device
-    for t in ts[1:]:
+def _one_derivative(backward):
+    """torch's once_differentiable where a second derivative could be asked for (create_graph), the bare function where not:
+    its context managers cost a small loss a tenth of its backward pass."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+def _same_device(first, *others):
+    _need_cuda(first)
+    dev = first.device
+    for t in others:
         if t is not None and t.device != dev:
+            _need_cuda(t)
             raise ValueError("tensors on different devices: %s and %s" % (dev, t.device))
     return dev
 
@@ -2709,21 +2721,25 @@ def _constant(name, t, shape):
     """A tensor that carries no gradient here, as contiguous fp32 of the given shape."""
     if t is None:
         return None
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s is a constant of this loss: detach it" % name)
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
     if not t.dtype.is_floating_point:
         raise ValueError("%s must be floating point (got %s)" % (name, t.dtype))
-    return t.detach().to(torch.float32).contiguous() if t.dtype != torch.float32 or not t.is_contiguous() else t
+    return t.detach().to(torch.float32).contiguous()
 
 
 def _index(name, t, shape):
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.dtype == torch.int64 and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int64, torch.int32):
         raise ValueError("%s must be int64 or int32 (got %s)" % (name, t.dtype))
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    return t.to(torch.int64).contiguous() if t.dtype != torch.int64 or not t.is_contiguous() else t
+    return t.to(torch.int64).contiguous()
 
 
 def _check_rows(logits):
@@ -2780,18 +2796,10 @@ def _ws_bytes(rows):
     return _WS_BASE + 16 * rows
 
 
-def _align16(n):
-    return (n + 15) // 16 * 16
-
-
-def _pieces(dev, *sizes):
-    """One allocation for what a call keeps or scribbles on: (tensor, address of each piece, 16-byte aligned)."""
-    buf = torch.empty(builtins.sum(map(_align16, sizes)), dtype=torch.uint8, device=dev)
-    at, out = buf.data_ptr(), [buf]
-    for n in sizes:
-        out.append(at)
-        at += _align16(n)
-    return out
+def _bytes(n, dev):
+    """One allocation for what a call keeps and scribbles on -> (tensor, its address)."""
+    buf = torch.empty(n, dtype=torch.uint8, device=dev)
+    return buf, buf.data_ptr()
 
 
 def _one_pass_grad(logits, want):
@@ -2827,7 +2835,7 @@ class TokenLogProbs(torch.autograd.Function):
         return (logp, ent) if entropy else logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, dlogp, dent=None):
         if dlogp is None and dent is None:
             return (None,) * 6
@@ -2866,25 +2874,29 @@ class DistillTopK(torch.autograd.Function):
         dev, K = x.device, ids.shape[-1]
         T = ids.numel() // K
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        buf, save, psum, ws = _pieces(dev, 16 * T, 4 * T * K, _ws_bytes(T))
+        buf, save = _bytes(16 * T + _ws_bytes(T) + 4 * T * K, dev)
+        ws = save + 16 * T
+        psum = ws + _ws_bytes(T)
         d = _one_pass_grad(logits, want_grad)
         _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, _p(ids), _p(t_logits),
                 _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), save if want_grad else None, psum, _p(d), ws)
         if want_grad:
             ctx.save_for_backward(x, ids, buf)
             ctx.grad = d
-        ctx.meta = (inv_temp, K, T, logits.shape)
+        ctx.meta = (inv_temp, K, psum - save, logits.shape)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, g):
         x, ids, buf = ctx.saved_tensors
-        inv_temp, K, T, shape = ctx.meta
+        inv_temp, K, at, shape = ctx.meta
         d, ready = _take_grad(ctx, x, shape)
-        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(buf), _p(buf) + _align16(16 * T), _p(g),
-                ready, _p(d))
+        _launch(x.device, "pv_distill_rows_bwd", *_row_args(x), inv_temp, _p(ids), K, _p(buf), _p(buf) + at, _p(g), ready, _p(d))
         return (d,) + (None,) * 8
+
+
+DISTILL_MAX = 256                # pv_distill_max_entries()
 
 
 def distill_topk(logits, teacher_ids, teacher_logits, labels=None, ignore_index=None, temperature=1.0, weight=1.0,
@@ -2899,12 +2911,11 @@ def distill_topk(logits, teacher_ids, teacher_logits, labels=None, ignore_index=
     names no word makes the loss NaN.  A coefficient belongs into `weight`: an upstream gradient other than 1 costs another
     pass over the rows."""
     _check_rows(logits)
-    lead = tuple(logits.shape[:-1])
-    K_max = _lib.load().pv_distill_max_entries()
-    if teacher_logits.dim() != logits.dim() or tuple(teacher_logits.shape[:-1]) != lead or teacher_logits.shape[-1] < 1:
-        raise ValueError("teacher_logits has shape %s, expected %s" % (tuple(teacher_logits.shape), lead + ("K",)))
-    if teacher_logits.shape[-1] > K_max:
-        raise ValueError("%d teacher entries a row, at most %d are taken" % (teacher_logits.shape[-1], K_max))
+    lead = logits.shape[:-1]
+    if teacher_logits.dim() != logits.dim() or teacher_logits.shape[:-1] != lead or teacher_logits.shape[-1] < 1:
+        raise ValueError("teacher_logits has shape %s, expected %s" % (tuple(teacher_logits.shape), tuple(lead) + ("K",)))
+    if teacher_logits.shape[-1] > DISTILL_MAX:
+        raise ValueError("%d teacher entries a row, at most %d are taken" % (teacher_logits.shape[-1], DISTILL_MAX))
     if teacher_logits.dtype not in _ROW_DTYPES:
         raise ValueError("teacher_logits must be float32, bfloat16 or float16 (got %s)" % teacher_logits.dtype)
     if teacher_logits.requires_grad and torch.is_grad_enabled():
@@ -2930,11 +2941,11 @@ class VocabPolicyLoss(torch.autograd.Function):
         x = _plain_rows(logits)
         dev, T = x.device, tokens.numel()
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
-        buf, save, ws = _pieces(dev, 16 * T, _ws_bytes(T))
+        buf, save = _bytes(16 * T + _ws_bytes(T), dev)
         d = _one_pass_grad(logits, want_grad)
         _launch(dev, "pv_policy_rows_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(old), _p(ref), _p(adv),
                 int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), save if want_grad else None,
-                _p(d), ws)
+                _p(d), save + 16 * T)
         if want_grad:
             ctx.save_for_backward(x, tokens, buf)
             ctx.grad = d
@@ -2943,7 +2954,7 @@ class VocabPolicyLoss(torch.autograd.Function):
         return loss, stats
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, g, _dstats):
         x, tokens, buf = ctx.saved_tensors
         ignore, inv_temp, shape = ctx.meta
@@ -2961,7 +2972,8 @@ class PolicyLoss(torch.autograd.Function):
         dev, T = x.device, tokens.numel()
         n1 = x.shape[1] if x.dim() == 2 else T
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
-        buf, dlp, ws = _pieces(dev, 4 * (T + 1), _ws_bytes(0))
+        buf, ws = _bytes(_ws_bytes(0) + 4 * (T + 1), dev)
+        dlp = ws + _ws_bytes(0)
         _launch(dev, "pv_policy_tokens_fwd", _p(x), _p(tokens), ignore, T // n1, n1, _p(old), _p(ref), _p(adv),
                 int(adv.numel() == T), lo, hi, kl, weight, word, _p(loss), _p(stats), dlp if want_grad else None, ws)
         if want_grad:
@@ -2971,18 +2983,17 @@ class PolicyLoss(torch.autograd.Function):
         return loss, stats
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, g, _dstats):
         buf, = ctx.saved_tensors
         d = torch.empty(ctx.shape, dtype=torch.float32, device=buf.device)
-        _launch(buf.device, "pv_policy_tokens_bwd", _p(buf), _p(g), d.numel(), _p(d))
+        _launch(buf.device, "pv_policy_tokens_bwd", _p(buf) + _ws_bytes(0), _p(g), d.numel(), _p(d))
         return (d,) + (None,) * 11
 
 
 def _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef):
     old, ref = _constant("old_logp", old_logp, shape), _constant("ref_logp", ref_logp, shape)
-    per_token = tuple(advantages.shape) == tuple(shape)
-    adv = _constant("advantages", advantages, shape if per_token or len(shape) < 2 else shape[:1])
+    adv = _constant("advantages", advantages, shape if len(shape) < 2 or advantages.shape == shape else shape[:1])
     clip_high = clip if clip_high is None else clip_high
     if not (clip >= 0 and clip_high >= 0):
         raise ValueError("the clip range must not be negative (got %r, %r)" % (clip, clip_high))
@@ -3001,7 +3012,7 @@ def vocab_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, ignor
     term, of "the clip decides" and of H.  old_logp, ref_logp and advantages are constants.  Dead rows (`ignore_index`) are
     not read.  A coefficient belongs into `weight`: an upstream gradient other than 1 costs another pass over the rows."""
     _check_rows(logits)
-    shape = tuple(logits.shape[:-1])
+    shape = logits.shape[:-1]
     if not 1 <= len(shape) <= 2:
         raise ValueError("logits must be [B, L, V] or [T, V] (got shape %s)" % (tuple(logits.shape),))
     tokens = _index("tokens", tokens, shape)
@@ -3020,9 +3031,9 @@ def policy_loss(logp, tokens, old_logp, advantages, ref_logp=None, ignore_index=
                 weight=1.0, avg_type="word"):
     """vocab_policy_loss from the tokens' log-probabilities `logp` [B, L] (or [T]), as token_logprobs or the fused vocabulary
     projection gives them; no entropy term.  -> (loss, stats), the last of the stats 0."""
-    shape = tuple(logp.shape)
+    shape = logp.shape
     if not 1 <= len(shape) <= 2 or logp.dtype != torch.float32:
-        raise ValueError("logp must be float32 [B, L] or [T] (got %s %s)" % (logp.dtype, shape))
+        raise ValueError("logp must be float32 [B, L] or [T] (got %s %s)" % (logp.dtype, tuple(shape)))
     tokens = _index("tokens", tokens, shape)
     old, ref, adv, lo, hi, kl = _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef)
     w, word = _avg(avg_type, weight, shape[0])
@@ -3043,9 +3054,9 @@ class PreferenceLoss(torch.autograd.Function):
         dev, P = xc.device, xc.shape[0]
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
-        buf, slope, ws = _pieces(dev, 4 * P, _ws_bytes(P))
+        buf, ws = _bytes(_ws_bytes(P) + 4 * P, dev)
         _launch(dev, "pv_preference_fwd", _p(xc), _p(ref_c), _p(labels_c), xc.shape[1], _p(xr), _p(ref_r), _p(labels_r),
-                xr.shape[1], P, ignore, beta, smoothing, weight, _p(loss), _p(rewards), slope, ws)
+                xr.shape[1], P, ignore, beta, smoothing, weight, _p(loss), _p(rewards), ws + _ws_bytes(P), ws)
         ctx.save_for_backward(labels_c, labels_r, buf)
         ctx.meta = (ignore, weight)
         rc, rr = rewards[0], rewards[1]
@@ -3053,14 +3064,14 @@ class PreferenceLoss(torch.autograd.Function):
         return loss, rc, rr
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, g, _drc, _drr):
         labels_c, labels_r, buf = ctx.saved_tensors
         ignore, weight = ctx.meta
         dc = torch.empty(labels_c.shape, dtype=torch.float32, device=buf.device)
         dr = torch.empty(labels_r.shape, dtype=torch.float32, device=buf.device)
         _launch(buf.device, "pv_preference_bwd", _p(labels_c), labels_c.shape[1], _p(labels_r), labels_r.shape[1],
-                labels_c.shape[0], ignore, _p(buf), weight, _p(g), _p(dc), _p(dr))
+                labels_c.shape[0], ignore, _p(buf) + _ws_bytes(labels_c.shape[0]), weight, _p(g), _p(dc), _p(dr))
         return (dc, dr) + (None,) * 8
 
 
@@ -3073,25 +3084,28 @@ class VocabPreferenceLoss(torch.autograd.Function):
         dev, P, Tc, Tr = xc.device, xc.shape[0], labels_c.numel(), labels_r.numel()
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
-        buf, slope, save_c, save_r, ws = _pieces(dev, 4 * P, 16 * Tc, 16 * Tr, _ws_bytes(P) + 4 * (Tc + Tr))
+        buf, save_c = _bytes(16 * (Tc + Tr) + _ws_bytes(P) + 4 * (Tc + Tr) + 4 * P, dev)
+        save_r = save_c + 16 * Tc
+        ws = save_r + 16 * Tr
+        slope = ws + _ws_bytes(P) + 4 * (Tc + Tr)
         ac, ar = _row_args(xc), _row_args(xr)
         _launch(dev, "pv_preference_rows_fwd", *ac, _p(labels_c), _p(ref_c), *ar[:2], *ar[3:], _p(labels_r), _p(ref_r), ignore,
                 inv_temp, beta, smoothing, weight, _p(loss), _p(rewards), slope, save_c if grad_c else None,
                 save_r if grad_r else None, ws)
         if grad_c or grad_r:
             ctx.save_for_backward(xc if grad_c else None, xr if grad_r else None, labels_c, labels_r, buf)
-        ctx.meta = (ignore, inv_temp, weight)
+        ctx.meta = (ignore, inv_temp, weight, slope - save_c)
         rc, rr = rewards[0], rewards[1]
         ctx.mark_non_differentiable(rc, rr)
         return loss, rc, rr
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_one_derivative
     def backward(ctx, g, _drc, _drr):
         xc, xr, labels_c, labels_r, buf = ctx.saved_tensors
-        ignore, inv_temp, weight = ctx.meta
-        slope = _p(buf)
-        save = slope + _align16(4 * labels_c.shape[0])
+        ignore, inv_temp, weight, at = ctx.meta
+        save = _p(buf)
+        slope = save + at
         out = []
         for x, labels, w in ((xc, labels_c, weight), (xr, labels_r, -weight)):
             d = None
@@ -3126,7 +3140,7 @@ def vocab_preference_loss(chosen_logits, chosen_labels, rejected_logits, rejecte
         if x.dim() != 3:
             raise ValueError("logits must be [P, L, V] (got shape %s)" % (tuple(x.shape),))
     _check_temp(inv_temp)
-    shape_c, shape_r = tuple(chosen_logits.shape[:2]), tuple(rejected_logits.shape[:2])
+    shape_c, shape_r = chosen_logits.shape[:2], rejected_logits.shape[:2]
     lc, lr, rc, rr = _preference_args(shape_c, shape_r, chosen_labels, rejected_labels, ref_chosen, ref_rejected, label_smoothing,
                                       avg_type)
     _same_device(chosen_logits, chosen_labels, rejected_logits, rejected_labels, ref_chosen, ref_rejected)
@@ -3151,8 +3165,8 @@ def preference_loss(chosen_logp, chosen_labels, rejected_logp, rejected_labels, 
     for name, t in (("chosen_logp", chosen_logp), ("rejected_logp", rejected_logp)):
         if t.dim() != 2 or t.dtype != torch.float32:
             raise ValueError("%s must be float32 [P, L] (got %s %s)" % (name, t.dtype, tuple(t.shape)))
-    lc, lr, rc, rr = _preference_args(tuple(chosen_logp.shape), tuple(rejected_logp.shape), chosen_labels, rejected_labels,
-                                      ref_chosen, ref_rejected, label_smoothing, avg_type)
+    lc, lr, rc, rr = _preference_args(chosen_logp.shape, rejected_logp.shape, chosen_labels, rejected_labels, ref_chosen,
+                                      ref_rejected, label_smoothing, avg_type)
     _same_device(chosen_logp, chosen_labels, rejected_logp, rejected_labels, ref_chosen, ref_rejected)
     P = chosen_logp.shape[0]
     if P == 0:

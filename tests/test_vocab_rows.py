@@ -100,5 +100,5 @@ def test_entry_points_refuse_on_the_host():
     assert lib.pv_preference_rows_fwd(p, 0, 2, 3, 15, 5, 5, p, None, p, 0, 0, 15, 5, 5, p, None, 0, 1.0, 0.1, 0.0, 1.0, p, p, p, p, p, p,
                                       None) == -1
     assert lib.pv_preference_rows_bwd(p, 0, 2, 3, 15, 5, 5, p, 0, 1.0, None, p, 1.0, p, p, None) == -1
-    assert lib.pv_distill_max_entries() == 256
+    assert lib.pv_distill_max_entries() == 256 == ops.DISTILL_MAX
     assert lib.pv_vocab_rows_ws_bytes(10) >= 160
