@@ -539,7 +539,15 @@ int pv_dropout_pack_bf16(const float* src, int n0, int n1, int n1p, int C, long 
 size_t pv_vocab_rows_ws_bytes(long rows);
 /* Whether rows of V words fit the one-pass form of the policy and distillation calls: forward with dlogits != NULL (and
  * save) writes the gradient for an upstream gradient of 1 as well, and backward with ready != 0 and the same dlogits leaves it
- * where *g is 1 and computes it afresh where it is not. */
+ * where *g is 1 and computes it afresh where it is not.  ld_bf16 > 0 (fp32 logits): that gradient as bf16 rows of ld_bf16
+ * words, V <= ld_bf16 < V + 64, zeros behind the V words: the operand of the products behind a projection (no backward call);
+ * perm (NULL: none) then says that row t of the logits and of the gradient is row perm[t] of everything else, a permutation
+ * that puts the dead rows, whose logits need not be there, last (pv_vocab_compact).
+ * pv_colsum_scaled_bf16: out[v] = *g * sum over T such rows, in a fixed order; ws: pv_colsum_scaled_ws_bytes(V).
+ * pv_scale_by_f32: x *= *g (n % 4 == 0, 16-byte aligned; no pass where *g is 1). */
+size_t pv_colsum_scaled_ws_bytes(int V);
+int pv_colsum_scaled_bf16(const void* P, long ld, long T, int V, const float* g, float* out, void* ws, void* stream);
+int pv_scale_by_f32(float* x, long n, const float* g, void* stream);
 int pv_vocab_rows_one_pass(int dtype, int V);
 /* logp[t] = log_softmax(logits * inv_temp)[t][tokens[t]]; entropy[t] (NULL: not wanted) of the same distribution.  Backward
  * for upstream gradients dlogp / dentropy [rows] (either may be NULL). */
@@ -556,18 +564,21 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
 int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                        int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
                        int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
-                       float* loss, float* stats, float* save, void* dlogits, void* ws, void* stream);
+                       float* loss, float* stats, float* save, void* dlogits, long ld_bf16,
+                       const int64_t* perm, void* ws, void* stream);
 int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                        int64_t ignore, float inv_temp, const float* save, const float* g, int ready, void* dlogits, void* stream);
 /* Distillation from a teacher's K top logits (t_ids int64 / t_logits [rows][K], K <= pv_distill_max_entries()): with p the
- * softmax of the row's teacher logits and q that of its logits, both at the temperature 1 / inv_temp,
- *   loss = scale / inv_temp^2 * sum over live rows of sum_j p_j (log p_j - log q[t_ids_j])
+ * softmax of the row's teacher logits at the temperature 1 / t_inv_temp and q that of its logits at 1 / inv_temp (the same,
+ * unless the logits carry a temperature of their own),
+ *   loss = scale / t_inv_temp^2 * sum over live rows of sum_j p_j (log p_j - log q[t_ids_j])
  * Entries of -inf do not count (their ids are not read as words); a row without any counts as dead except for the live count.
  * labels NULL: every row is live.  psum: [rows][K] floats kept for the backward call. */
 int pv_distill_max_entries(void);
 int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
-                        int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
-                        float weight, int word, float* loss, float* save, float* psum, void* dlogits, void* ws, void* stream);
+                        int64_t ignore, float inv_temp, float t_inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype,
+                        int K, float weight, int word, float* loss, float* save, float* psum, void* dlogits, long ld_bf16,
+                        const int64_t* perm, void* ws, void* stream);
 int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp,
                         const int64_t* t_ids, int K, const float* save, const float* psum, const float* g, int ready,
                         void* dlogits, void* stream);

@@ -151,10 +151,13 @@ SIGNATURES = {
     "pv_vocab_rows_one_pass": (i32, [i32, i32]),
     "pv_token_logp_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp]),
     "pv_token_logp_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, vp, vp]),
-    "pv_policy_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, i32, f32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp, vp]),
+    "pv_policy_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, vp, i32, f32, f32, f32, f32, f32, i32, vp, vp, vp, vp, lng, vp, vp, vp]),
     "pv_policy_rows_bwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, vp, vp]),
     "pv_distill_max_entries": (i32, []),
-    "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp, vp]),
+    "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, lng, vp, vp, vp]),
+    "pv_colsum_scaled_ws_bytes": (sz, [i32]),
+    "pv_colsum_scaled_bf16": (i32, [vp, lng, lng, i32, vp, vp, vp, vp]),
+    "pv_scale_by_f32": (i32, [vp, lng, vp, vp]),
     "pv_distill_rows_bwd": (i32, _ROWS + [f32, vp, i32, vp, vp, vp, i32, vp, vp]),
     "pv_policy_tokens_fwd": (i32, [vp, vp, i64, lng, i32, vp, vp, vp, i32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),
     "pv_policy_tokens_bwd": (i32, [vp, vp, lng, vp, vp]),

@@ -124,7 +124,8 @@ def token_log_probs(net_output, labels, padding_idx):
 class TopKDistill(_Loss):
     """Distillation from a teacher's top logits (ops.distill_topk): forward(net_output, labels, teacher_ids, teacher_logits)
     with teacher_ids / teacher_logits [B, L, K] -> loss.  avg_type as NLLEntropy's: 'seq' = sum / batch, 'word' = token mean,
-    None = sum.  A DeferredLogProbs is materialised: the teacher's softmax needs the whole row's statistics and K words of it."""
+    None = sum.  A DeferredLogProbs is taken from its projection on (ops.projected_distill_topk): no log-probabilities are
+    written, and no gradient of them."""
 
     def __init__(self, padding_idx, config, temperature=1.0, weight=1.0, avg_type="seq"):
         super().__init__()
@@ -134,6 +135,10 @@ class TopKDistill(_Loss):
 
     def forward(self, net_output, labels, teacher_ids, teacher_logits):
         if isinstance(net_output, DeferredLogProbs):
+            if ops.projection_fits(net_output.size(2)):
+                hid, w, b, inv_temp = net_output.projection()
+                return ops.projected_distill_topk(hid, w, b, teacher_ids, teacher_logits, labels, self.padding_idx, inv_temp,
+                                                  self.temperature, self.weight, self.avg_type)
             net_output = net_output.materialize()
         return ops.distill_topk(net_output, teacher_ids, teacher_logits, labels, self.padding_idx, self.temperature,
                                 self.weight, self.avg_type)
@@ -142,7 +147,8 @@ class TopKDistill(_Loss):
 class ClippedPolicyLoss(_Loss):
     """Clipped policy loss with a KL term and an entropy bonus (ops.vocab_policy_loss): forward(net_output, labels, old_logp,
     advantages, ref_logp=None) -> (loss, stats), labels = the sampled tokens [B, L], padded.  A DeferredLogProbs goes through
-    the fused vocabulary projection (no [B, L, V] tensor) unless there is an entropy bonus, which needs the rows."""
+    the fused vocabulary projection (no [B, L, V] tensor), or with an entropy bonus, which needs the rows, through
+    ops.projected_policy_loss."""
 
     def __init__(self, padding_idx, config, clip=0.2, clip_high=None, kl_coef=0.0, ent_coef=0.0, weight=1.0, avg_type="word"):
         super().__init__()
@@ -156,6 +162,11 @@ class ClippedPolicyLoss(_Loss):
             if self.ent_coef == 0:
                 return ops.policy_loss(net_output.token_logp(labels, self.padding_idx), labels, old_logp, advantages, ref_logp,
                                        self.padding_idx, self.clip, self.clip_high, self.kl_coef, self.weight, self.avg_type)
+            if ops.projection_fits(net_output.size(2)):
+                hid, w, b, inv_temp = net_output.projection()
+                return ops.projected_policy_loss(hid, w, b, labels, old_logp, advantages, ref_logp, self.padding_idx, inv_temp,
+                                                 self.clip, self.clip_high, self.kl_coef, self.ent_coef, self.weight,
+                                                 self.avg_type)
             net_output = net_output.materialize()
         return ops.vocab_policy_loss(net_output, labels, old_logp, advantages, ref_logp, self.padding_idx, 1.0, self.clip,
                                      self.clip_high, self.kl_coef, self.ent_coef, self.weight, self.avg_type)

@@ -26,6 +26,7 @@ enum { HEAD_TOKEN = 0, HEAD_POLICY = 1, HEAD_DISTILL = 2 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(1))) piece_t { u32x4 v; };     // 16 bytes at any address
+struct __attribute__((packed, aligned(1))) half_piece_t { uint32_t v[2]; };
 
 // (a copy of the element: __builtin_bit_cast of an element of a vector register reads element 0)
 __device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -150,9 +151,24 @@ __device__ __forceinline__ float slope(float z, const float4& w, float k) {
   const float x = (z - w.x) * k, e = exp2_(x);
   return B ? e * (w.y + w.z * fmaxf(x, kFloorX)) : e * w.y;
 }
-// the gradient of one piece of a row whose first word is v; y: the word that gets d on top (none: negative)
-template <class E, bool B>
-__device__ __forceinline__ u32x4 slope_piece(u32x4 raw, int v, const float4& w, float k, int y, float d) {
+// the N values of a piece of the input as elements of the output type O
+template <class E, class O>
+__device__ __forceinline__ void store_values(typename O::type* p, const float (&z)[E::N]) {
+  if constexpr (E::N == O::N) {
+    store_piece(p, O::pack(z));
+  } else {                                         // four fp32 values to four bf16 ones
+    half_piece_t h = {{pack2bf(z[0], z[1]), pack2bf(z[2], z[3])}};
+    *(half_piece_t*)p = h;
+  }
+}
+template <class E, class O>
+__device__ __forceinline__ void store_zeros(typename O::type* p) {
+  const float z[E::N] = {};
+  store_values<E, O>(p, z);
+}
+// the gradient of one piece of a row whose first word is v, to out; y: the word that gets d on top (none: negative)
+template <class E, class O, bool B>
+__device__ __forceinline__ void slope_piece(typename O::type* out, u32x4 raw, int v, const float4& w, float k, int y, float d) {
   float z[E::N];
   E::unpack(raw, z);
 #pragma unroll
@@ -161,7 +177,7 @@ __device__ __forceinline__ u32x4 slope_piece(u32x4 raw, int v, const float4& w, 
 #pragma unroll
     for (int n = 0; n < E::N; ++n) z[n] += v + n == y ? d : 0.f;
   }
-  return E::pack(z);
+  store_values<E, O>(out + v, z);
 }
 
 // x - ln(s) to about half a unit of the result: ln s = n ln2 + ln f with the two halves of ln2 kept apart, the rounding of
@@ -194,6 +210,7 @@ struct Rows {
   float c, k;                // 1 / temperature, c * log2(e)
   const int64_t* labels;     // NULL: every row is live and there is no label
   int64_t ignore;
+  const int64_t* perm;       // rows_once_kernel: row t of the logits is row perm[t] of everything else (NULL: t)
 };
 struct Policy {
   const float *old_lp, *ref_lp, *adv;      // ref_lp NULL: no KL term; adv [T] or [T / n1]
@@ -205,6 +222,7 @@ struct Distill {
   const void* t_logits;      // [T][K]
   int K, dtype;
   float* psum;               // [T][K]: the teacher's probability of the entry's word, duplicates added up
+  float c, k;                // 1 / temperature of the loss and of the teacher, c * log2(e)
 };
 struct Scale {
   float weight;              // of the loss, divided by *count where count != NULL (at least 1)
@@ -285,7 +303,7 @@ __device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, 
   r.empty = mx == -__builtin_inff();
   float sum = 0.f, zr = -__builtin_inff(), bad = 0.f;
   for (int j = lane; j < h.K; j += 64) {
-    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * a.k);
+    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * h.k);
     sum += p;
     if (p > 0.f) {
       if (l.id[j] < 0)
@@ -300,8 +318,8 @@ __device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, 
   const float inv = r.empty ? 0.f : 1.f / sum;
   float acc = 0.f;
   for (int j = lane; j < h.K; j += 64) {
-    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * a.k) * inv;
-    if (p > 0.f && l.id[j] >= 0) acc += p * (minus_log((x - mx) * a.c, sum) - a.c * (E::up(row[l.id[j]]) - r.zref));
+    const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * h.k) * inv;
+    if (p > 0.f && l.id[j] >= 0) acc += p * (minus_log((x - mx) * h.c, sum) - a.c * (E::up(row[l.id[j]]) - r.zref));
     l.p[j] = p;
   }
   r.acc = wave_sum(acc);
@@ -343,7 +361,7 @@ __device__ __forceinline__ void accumulate(Stat& st, const float (&z)[N], float 
 
 // the row's loss terms (stored by one thread, where `first`) and {m, a, b, d}, the coefficients of its gradient
 template <int HEAD>
-__device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, const RowIn& in, const Teacher& te, const FwdOut& o,
+__device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, float tau, const RowIn& in, const Teacher& te, const FwdOut& o,
                                              long t, Stat st, float zy, bool bad, bool first) {
   const float nan = __builtin_nanf("");
   const float inv = 1.f / st.s, ln2 = 0.69314718056f;
@@ -363,12 +381,11 @@ __device__ __forceinline__ float4 finish_row(const Rows& a, const Policy& hp, co
     const float w = in.scale, g = w * q.dlp, h = -w * hp.ent;
     return make_float4(st.m, -a.c * inv * (g - h * ln2 * st.ex * inv), -a.c * inv * h * ln2, a.c * g);
   } else {
-    const float tau = 1.f / a.c;
     if (first) {
       const float loss = te.bad ? nan : te.acc + (a.c * (st.m - te.zref) - minus_log(0.f, st.s));
       o.rowout[t] = make_float4(te.empty ? 0.f : tau * tau * loss, 0.f, 0.f, 0.f);
     }
-    const float w = in.scale * tau;               // tau^2 / tau
+    const float w = in.scale * tau * tau * a.c;
     return make_float4(te.empty ? kDead : st.m, te.bad ? nan : w * inv, 0.f, -w);
   }
 }
@@ -472,21 +489,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void rows_fwd_kernel(Rows a, P
   }
   st = P::template join<ENT>(st, a.k, part);
   if (tid == 0) {
-    const float4 w = finish_row<HEAD>(a, hp, in, te, o, t, st, zy, bad, true);
+    const float4 w = finish_row<HEAD>(a, hp, 1.f / hd.c, in, te, o, t, st, zy, bad, true);
     if (o.save) o.save[t] = w;
   }
 }
 
-template <class E, bool B, int NT, int CH>
-__device__ __forceinline__ void write_once(u32x4 (&raw)[CH], typename E::type* out, int tid, const Split<E>& sp,
+template <class E, class O, bool B, int NT, int CH>
+__device__ __forceinline__ void write_once(u32x4 (&raw)[CH], typename O::type* out, int tid, const Split<E>& sp,
                                            const float4& w, float k, int y, float d) {
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = tid + i * NT;
     keep_packed(raw[i]);
-    const int v = sp.head + c * E::N;
-    if (c < sp.full) store_piece(out + v, slope_piece<E, B>(raw[i], v, w, k, y, d));
+    if (c < sp.full) slope_piece<E, O, B>(out, raw[i], sp.head + c * E::N, w, k, y, d);
   }
+}
+template <class E, class O>
+__device__ __forceinline__ void zero_row(typename O::type* out, int tid, int step, const Split<E>& sp, int V) {
+  for (int i = tid; i < sp.full; i += step) store_zeros<E, O>(out + sp.head + (long)i * E::N);
+  const int rest = sp.edge(tid, V);
+  if (rest < V) out[rest] = O::down(0.f);
 }
 
 // Loss and gradient of a row in one pass: the row stays in its threads' registers (CH pieces each) between its statistics and
@@ -494,25 +516,27 @@ __device__ __forceinline__ void write_once(u32x4 (&raw)[CH], typename E::type* o
 // twice.  Each thread runs its own maximum and sums while its pieces arrive; one exchange through shared memory gives every
 // wave the row's.  WAVES a SIMD bound the registers so that a CU holds several rows: while one waits for memory another one
 // computes.
-template <class E, int HEAD, int NT, int CH, int WAVES>
+// The gradient has the logits' type E, or is bf16 for fp32 logits: the operand of the products behind a projection, whose rows
+// are ldg elements apart with zeros behind the V words.
+template <class E, class O, int HEAD, int NT, int CH, int WAVES>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(Rows a, Policy hp, Distill hd, Scale sc, FwdOut o,
-                                                                           typename E::type* __restrict__ grad) {
+                                                                           typename O::type* __restrict__ grad, long ldg) {
   typedef Place<NT> P;
   const long t = P::row();
   const int tid = P::tid();
   if (P::R > 1 && t >= a.T) return;
-  typename E::type* out = grad + t * a.V;
-  const Split<E> sp(out, a.V);
+  typename O::type* out = grad + t * ldg;
+  const Split<E> sp(E::N == O::N ? (const void*)out : (const void*)row_of<E>(a, t), a.V);
   const int full = sp.full, rest = sp.edge(tid, a.V);
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  const int64_t y = a.labels ? a.labels[t] : -1;
+  if (E::N != O::N && a.V + tid < ldg) out[a.V + tid] = O::down(0.f);      // fewer than 64 words
+  const long src = a.perm ? a.perm[t] : t;
+  const int64_t y = a.labels ? a.labels[src] : -1;
   if (a.labels && y == a.ignore) {
-    for (int i = tid; i < full; i += NT) store_piece(out + sp.head + (long)i * E::N, zero);
-    if (rest < a.V) out[rest] = E::down(0.f);
+    zero_row<E, O>(out, tid, NT, sp, a.V);
     if (tid == 0) dead_row<HEAD>(o, t);
     return;
   }
-  const RowIn in = load_row_in<HEAD>(a, hp, sc, t);
+  const RowIn in = load_row_in<HEAD>(a, hp, sc, src);
   const typename E::type* row = row_of<E>(a, t);
   u32x4 raw[CH];
 #pragma unroll
@@ -527,7 +551,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
   TeacherList& list = lists[HEAD == HEAD_DISTILL ? P::slot() : 0];
   Teacher te = {0.f, 0.f, false, false};
   if (HEAD == HEAD_DISTILL && tid < 64) {
-    te = teacher_row<E>(a, hd, t, row, tid, list);
+    te = teacher_row<E>(a, hd, src, row, tid, list);
     if (P::W > 1 && tid == 0) {
       flags[0] = te.empty;
       flags[1] = te.bad;
@@ -551,24 +575,23 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
     te.empty = flags[0];
     te.bad = flags[1];
   }
-  const float4 w = finish_row<HEAD>(a, hp, in, te, o, t, st, zy, bad, tid == 0);
+  const float4 w = finish_row<HEAD>(a, hp, 1.f / hd.c, in, te, o, t, st, zy, bad, tid == 0);
   if (tid == 0) o.save[t] = w;
   if (HEAD == HEAD_DISTILL && w.x == kDead) {
-    for (int i = tid; i < full; i += NT) store_piece(out + sp.head + (long)i * E::N, zero);
-    if (rest < a.V) out[rest] = E::down(0.f);
+    zero_row<E, O>(out, tid, NT, sp, a.V);
     return;
   }
   const int yy = HEAD == HEAD_POLICY ? (int)y : -1;
   if (HEAD == HEAD_POLICY && w.z != 0.f)
-    write_once<E, true, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
+    write_once<E, O, true, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
   else
-    write_once<E, false, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
-  if (rest < a.V) out[rest] = E::down(slope<HEAD == HEAD_POLICY>(zr, w, a.k) + (rest == yy ? w.w : 0.f));
+    write_once<E, O, false, NT, CH>(raw, out, tid, sp, w, a.k, yy, w.w);
+  if (rest < a.V) out[rest] = O::down(slope<HEAD == HEAD_POLICY>(zr, w, a.k) + (rest == yy ? w.w : 0.f));
   if (HEAD == HEAD_DISTILL) {
     P::sync();                                     // the list's words are written again, after the sweep
     for (int j = tid; j < hd.K; j += NT) {
       const int id = list.id[j];
-      if (id >= 0) out[id] = E::down(slope<false>(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
+      if (id >= 0) out[id] = O::down(slope<false>(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
     }
   }
 }
@@ -594,10 +617,8 @@ __device__ __forceinline__ void sweep_grad(const typename E::type* row, typename
     for (int i = 0; i < 4; ++i)
       if (c + i * NT < end) raw[i] = load_piece(row + head + (long)(c + i * NT) * E::N);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = head + (c + i * NT) * E::N;
-      if (c + i * NT < end) store_piece(out + v, slope_piece<E, B>(raw[i], v, w, k, y, d));
-    }
+    for (int i = 0; i < 4; ++i)
+      if (c + i * NT < end) slope_piece<E, E, B>(out, raw[i], head + (c + i * NT) * E::N, w, k, y, d);
   }
 }
 
@@ -633,8 +654,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, 8) void rows_grad_kernel(Rows 
       if (HEAD == HEAD_POLICY && w.x != kDead) y = (int)a.labels[t];
     }
     if (w.x == kDead) {
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-      for (int c = c0 + tid; c < c1; c += NT) store_piece(out + sp.head + (long)c * E::N, zero);
+      for (int c = c0 + tid; c < c1; c += NT) store_zeros<E, E>(out + sp.head + (long)c * E::N);
       if (rest < a.V) out[rest] = E::down(0.f);
       continue;
     }
@@ -773,6 +793,61 @@ __global__ __launch_bounds__(256) void add_counts_kernel(const float* __restrict
   if (threadIdx.x == 0) out[0] = (float)v[0];
 }
 
+// ---- behind a projection: column sums of a bf16 gradient, results times a device scalar ------------------------------------
+// Columns in pairs, 128 to a workgroup; its four waves take a quarter each of a share of the rows, and a second launch adds
+// the shares in order.
+constexpr int kColShares = 64;
+__global__ __launch_bounds__(256) void colsum_part_kernel(const uint32_t* __restrict__ P, long ld2, long T, int V,
+                                                          float* __restrict__ part) {
+  __shared__ float2 sh[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pair = blockIdx.x * 64 + lane;
+  const long each = (T + gridDim.y - 1) / gridDim.y, t0 = blockIdx.y * each, t1 = t0 + each < T ? t0 + each : T;
+  float2 s = make_float2(0.f, 0.f);
+  if (2 * pair < V) {
+    for (long t = t0 + wave; t < t1; t += 4 * 8) {
+      uint32_t r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = t + 4 * i < t1 ? P[(t + 4 * i) * ld2 + pair] : 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s.x += as_float(r[i] << 16);
+        s.y += as_float(r[i] & 0xffff0000u);
+      }
+    }
+  }
+  sh[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || 2 * pair >= V) return;
+  for (int w = 1; w < 4; ++w) {
+    s.x += sh[w][lane].x;
+    s.y += sh[w][lane].y;
+  }
+  part[blockIdx.y * (long)V + 2 * pair] = s.x;
+  if (2 * pair + 1 < V) part[blockIdx.y * (long)V + 2 * pair + 1] = s.y;
+}
+__global__ __launch_bounds__(64) void colsum_join_kernel(const float* __restrict__ part, int V, const float* __restrict__ g,
+                                                         float* __restrict__ out) {
+  const int v = blockIdx.x * 64 + threadIdx.x;
+  if (v >= V) return;
+  float s = 0.f;
+  for (int i0 = 0; i0 < kColShares; i0 += 16) {    // sixteen shares in flight
+    float r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = part[(i0 + i) * (long)V + v];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += r[i];
+  }
+  out[v] = s * *g;
+}
+__global__ __launch_bounds__(256) void scale_by_kernel(float4* __restrict__ x, long n4, const float* __restrict__ g) {
+  const float w = *g;
+  if (w == 1.f) return;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n4; i += gridDim.x * 256L) {
+    float4 v = x[i];
+    x[i] = make_float4(v.x * w, v.y * w, v.z * w, v.w * w);
+  }
+}
+
 // ---- policy loss from log-probabilities ------------------------------------------------------------------------------------
 // Latency bound: a few bytes a token.  One launch up to 4096 tokens, and one more that adds the workgroups' sums beyond.
 __global__ __launch_bounds__(1024) void policy_tokens_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels,
@@ -909,7 +984,7 @@ int check_count(const char* who, long n) {
   return PV_ERR_LIMIT;
 }
 Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, const int64_t* labels, int64_t ignore, float c) {
-  return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore};
+  return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore, nullptr};
 }
 
 inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
@@ -947,16 +1022,16 @@ int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, co
 // rows) 4.8, 1024 x 12 (one row) 4.2; V = 131071, bf16: 1024 x 16 3.9, which still beats two passes over memory (2.4).  Keeping
 // part of such rows in shared memory to hold two of them gained nothing (512 x 23 + 9: 3.6, its registers spill).
 constexpr int kOncePieces = 1024 * 20;            // of a row that the one-pass kernel holds
-template <class E, int HEAD>
-int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad,
+template <class E, class O, int HEAD>
+int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad, long ldg,
                       hipStream_t st) {
   const int pieces = a.V / E::N;
-  typename E::type* g = (typename E::type*)grad;
+  typename O::type* g = (typename O::type*)grad;
 #define PV_ONCE(NT, CH, WAVES)                                                                                  \
   if (pieces <= NT * CH) {                                                                                      \
     typedef Place<NT> P;                                                                                        \
-    rows_once_kernel<E, HEAD, NT, CH, WAVES>                                                                    \
-        <<<dim3((unsigned)((a.T + P::R - 1) / P::R)), dim3(NT * P::R), 0, st>>>(a, hp, hd, sc, o, g);            \
+    rows_once_kernel<E, O, HEAD, NT, CH, WAVES>                                                                 \
+        <<<dim3((unsigned)((a.T + P::R - 1) / P::R)), dim3(NT * P::R), 0, st>>>(a, hp, hd, sc, o, g, ldg);       \
     PV_LAUNCH_CHECK("rows_once_kernel");                                                                        \
     return PV_OK;                                                                                               \
   }
@@ -980,10 +1055,18 @@ int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const 
 }
 template <int HEAD>
 int launch_once(int dtype, const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad,
-                hipStream_t st) {
-  if (dtype == PV_DTYPE_F32) return launch_once_typed<F32, HEAD>(a, hp, hd, sc, o, grad, st);
-  if (dtype == PV_DTYPE_BF16) return launch_once_typed<BF16, HEAD>(a, hp, hd, sc, o, grad, st);
-  return launch_once_typed<F16, HEAD>(a, hp, hd, sc, o, grad, st);
+                long ldg, hipStream_t st) {
+  if (ldg > 0) return launch_once_typed<F32, BF16, HEAD>(a, hp, hd, sc, o, grad, ldg, st);
+  if (dtype == PV_DTYPE_F32) return launch_once_typed<F32, F32, HEAD>(a, hp, hd, sc, o, grad, a.V, st);
+  if (dtype == PV_DTYPE_BF16) return launch_once_typed<BF16, BF16, HEAD>(a, hp, hd, sc, o, grad, a.V, st);
+  return launch_once_typed<F16, F16, HEAD>(a, hp, hd, sc, o, grad, a.V, st);
+}
+int check_gradient(const char* who, int dtype, int V, const void* save, const void* dlogits, long ld_bf16, const void* perm) {
+  PV_REQUIRE(!perm || ld_bf16 > 0, "%s: an order of the rows goes with a bf16 gradient", who);
+  PV_REQUIRE(!dlogits || (save && pv_vocab_rows_one_pass(dtype, V)), "%s: no gradient in the forward pass here", who);
+  PV_REQUIRE(ld_bf16 == 0 || (dlogits && dtype == PV_DTYPE_F32 && ld_bf16 >= V && ld_bf16 - V < 64),
+             "%s: a bf16 gradient needs fp32 logits and rows of V to V + 63 words", who);
+  return PV_OK;
 }
 
 template <class E, int HEAD>
@@ -1066,14 +1149,16 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
 int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,
                        int64_t ignore, float inv_temp, const float* old_logp, const float* ref_logp, const float* adv,
                        int adv_per_token, float clip_lo, float clip_hi, float kl_coef, float ent_coef, float weight, int word,
-                       float* loss, float* stats, float* save, void* dlogits, void* ws, void* stream) {
-  const int rc = check_rows("pv_policy_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+                       float* loss, float* stats, float* save, void* dlogits, long ld_bf16,
+                       const int64_t* perm, void* ws, void* stream) {
+  int rc = check_rows("pv_policy_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc == PV_OK) rc = check_gradient("pv_policy_rows_fwd", dtype, V, save, dlogits, ld_bf16, perm);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(tokens && old_logp && adv && loss && stats && ws, "pv_policy_rows_fwd: null argument");
   PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_rows_fwd: the clip range is empty");
-  PV_REQUIRE(!dlogits || (save && pv_vocab_rows_one_pass(dtype, V)), "pv_policy_rows_fwd: no gradient in the forward pass here");
   hipStream_t st = (hipStream_t)stream;
-  const Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  Rows a = make_rows(logits, n0, n1, s0, s1, V, tokens, ignore, inv_temp);
+  a.perm = perm;
   float4* rowout = (float4*)ws;
   Sum5* part = (Sum5*)(rowout + a.T);
   Scale sc = {weight, nullptr};
@@ -1085,7 +1170,7 @@ int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, 
   }
   const Policy hp = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, ent_coef};
   const FwdOut o = {nullptr, nullptr, rowout, (float4*)save};
-  const int r = dlogits ? launch_once<HEAD_POLICY>(dtype, a, hp, Distill{}, sc, o, dlogits, st)
+  const int r = dlogits ? launch_once<HEAD_POLICY>(dtype, a, hp, Distill{}, sc, o, dlogits, ld_bf16, st)
                         : launch_fwd<HEAD_POLICY, true>(dtype, a, hp, Distill{}, sc, o, st);
   if (r != PV_OK) return r;
   return launch_sum(rowout, tokens, ignore, a.T, part, Result{kl_coef, ent_coef, weight, word, loss, stats, nullptr}, st);
@@ -1104,21 +1189,24 @@ int pv_policy_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0, 
 int pv_distill_max_entries(void) { return kTeacherMax; }
 
 int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* labels,
-                        int64_t ignore, float inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype, int K,
-                        float weight, int word, float* loss, float* save, float* psum, void* dlogits, void* ws, void* stream) {
-  const int rc = check_rows("pv_distill_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+                        int64_t ignore, float inv_temp, float t_inv_temp, const int64_t* t_ids, const void* t_logits, int t_dtype,
+                        int K, float weight, int word, float* loss, float* save, float* psum, void* dlogits, long ld_bf16,
+                        const int64_t* perm, void* ws, void* stream) {
+  int rc = check_rows("pv_distill_rows_fwd", logits, dtype, n0, n1, s0, s1, V, inv_temp);
+  if (rc == PV_OK) rc = check_gradient("pv_distill_rows_fwd", dtype, V, save, dlogits, ld_bf16, perm);
   if (rc != PV_OK) return rc;
   PV_REQUIRE(t_ids && t_logits && loss && psum && ws, "pv_distill_rows_fwd: null argument");
   PV_REQUIRE(t_dtype == PV_DTYPE_F32 || t_dtype == PV_DTYPE_BF16 || t_dtype == PV_DTYPE_F16,
              "pv_distill_rows_fwd: unknown teacher dtype %d", t_dtype);
   PV_REQUIRE(K > 0, "pv_distill_rows_fwd: no teacher entries");
-  PV_REQUIRE(!dlogits || (save && pv_vocab_rows_one_pass(dtype, V)), "pv_distill_rows_fwd: no gradient in the forward pass here");
+  PV_REQUIRE(t_inv_temp > 0.f && t_inv_temp < __builtin_inff(), "pv_distill_rows_fwd: the teacher's inverse temperature must be positive and finite");
   if (K > kTeacherMax) {
     pv_set_error("pv_distill_rows_fwd: %d teacher entries are beyond the limit of %d", K, kTeacherMax);
     return PV_ERR_LIMIT;
   }
   hipStream_t st = (hipStream_t)stream;
-  const Rows a = make_rows(logits, n0, n1, s0, s1, V, labels, ignore, inv_temp);
+  Rows a = make_rows(logits, n0, n1, s0, s1, V, labels, ignore, inv_temp);
+  a.perm = perm;
   float4* rowout = (float4*)ws;
   Sum5* part = (Sum5*)(rowout + a.T);
   Scale sc = {weight, nullptr};
@@ -1129,9 +1217,9 @@ int pv_distill_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0,
     if (r != PV_OK) return r;
     sc.count = count;
   }
-  const Distill hd = {t_ids, t_logits, K, t_dtype, psum};
+  const Distill hd = {t_ids, t_logits, K, t_dtype, psum, t_inv_temp, (float)((double)t_inv_temp * 1.4426950408889634)};
   const FwdOut o = {nullptr, nullptr, rowout, (float4*)save};
-  const int r = dlogits ? launch_once<HEAD_DISTILL>(dtype, a, Policy{}, hd, sc, o, dlogits, st)
+  const int r = dlogits ? launch_once<HEAD_DISTILL>(dtype, a, Policy{}, hd, sc, o, dlogits, ld_bf16, st)
                         : launch_fwd<HEAD_DISTILL, false>(dtype, a, Policy{}, hd, sc, o, st);
   if (r != PV_OK) return r;
   return launch_sum(rowout, labels, ignore, a.T, part, Result{0.f, 0.f, weight, word, loss, nullptr, nullptr}, st);
@@ -1144,8 +1232,30 @@ int pv_distill_rows_bwd(const void* logits, int dtype, long n0, int n1, long s0,
   if (rc != PV_OK) return rc;
   PV_REQUIRE(t_ids && save && psum && g && dlogits && K > 0 && K <= kTeacherMax, "pv_distill_rows_bwd: bad argument");
   const Rows a = make_rows(logits, n0, n1, s0, s1, V, nullptr, 0, inv_temp);
-  return launch_grad<HEAD_DISTILL>(dtype, a, Distill{t_ids, nullptr, K, 0, (float*)psum},
+  return launch_grad<HEAD_DISTILL>(dtype, a, Distill{t_ids, nullptr, K, 0, (float*)psum, 0.f, 0.f},
                                    Grad{(const float4*)save, nullptr, nullptr, nullptr, 0.f, g, dlogits, ready}, (hipStream_t)stream);
+}
+
+size_t pv_colsum_scaled_ws_bytes(int V) { return V > 0 ? (size_t)kColShares * V * sizeof(float) : 0; }
+
+int pv_colsum_scaled_bf16(const void* P, long ld, long T, int V, const float* g, float* out, void* ws, void* stream) {
+  PV_REQUIRE(P && g && out && ws && T > 0 && V > 0 && ld >= V, "pv_colsum_scaled_bf16: bad argument");
+  PV_REQUIRE(ld % 2 == 0 && ((uintptr_t)P & 3) == 0, "pv_colsum_scaled_bf16: rows must start at even elements");
+  hipStream_t st = (hipStream_t)stream;
+  colsum_part_kernel<<<dim3(cdiv(V, 128), kColShares), dim3(256), 0, st>>>((const uint32_t*)P, ld / 2, T, V, (float*)ws);
+  PV_LAUNCH_CHECK("colsum_part_kernel");
+  colsum_join_kernel<<<dim3(cdiv(V, 64)), dim3(64), 0, st>>>((const float*)ws, V, g, out);
+  PV_LAUNCH_CHECK("colsum_join_kernel");
+  return PV_OK;
+}
+
+int pv_scale_by_f32(float* x, long n, const float* g, void* stream) {
+  PV_REQUIRE(x && g && n >= 0 && n % 4 == 0 && ((uintptr_t)x & 15) == 0, "pv_scale_by_f32: n must be a multiple of 4, x 16-byte aligned");
+  if (n == 0) return PV_OK;
+  const long want = (n / 4 + 255) / 256;
+  scale_by_kernel<<<dim3((unsigned)(want > 1024 ? 1024 : want)), dim3(256), 0, (hipStream_t)stream>>>((float4*)x, n / 4, g);
+  PV_LAUNCH_CHECK("scale_by_kernel");
+  return PV_OK;
 }
 
 int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignore, long n0, int n1, const float* old_logp,

@@ -146,11 +146,16 @@ class DeferredLogProbs(object):
             return -nll.view(L, self.layout[2])[:, :B].t()
         return -nll.view(B, L)
 
+    def projection(self):
+        """(hid, weight, bias, inv_temp) of the log-probabilities, the output dropout applied."""
+        hid = self.hid if self.drop is None else ops.DropoutFn.apply(self.hid, *self.drop)
+        return hid, self.weight, self.bias, self.inv_temp
+
     # -- dense fallback: behaves like the reference's tensor ---------------------------------------------------
     def materialize(self):
         if self._dense is None:
             B, L, H = self.hid.shape
-            hid = self.hid if self.drop is None else ops.DropoutFn.apply(self.hid, *self.drop)
+            hid = self.projection()[0]
             flat = ops.VocabLogProbDense.apply(hid.reshape(B * L, H), self.weight, self.bias, self.inv_temp)
             self._dense = flat.view(B, L, -1)
         return self._dense

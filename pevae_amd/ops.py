@@ -2878,8 +2878,8 @@ class DistillTopK(torch.autograd.Function):
         ws = save + 16 * T
         psum = ws + _ws_bytes(T)
         d = _one_pass_grad(logits, want_grad)
-        _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, _p(ids), _p(t_logits),
-                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), save if want_grad else None, psum, _p(d), ws)
+        _launch(dev, "pv_distill_rows_fwd", *_row_args(x), _p(labels), ignore, inv_temp, inv_temp, _p(ids), _p(t_logits),
+                _ROW_DTYPES[t_logits.dtype], K, weight, word, _p(loss), save if want_grad else None, psum, _p(d), 0, None, ws)
         if want_grad:
             ctx.save_for_backward(x, ids, buf)
             ctx.grad = d
@@ -2899,6 +2899,20 @@ class DistillTopK(torch.autograd.Function):
 DISTILL_MAX = 256                # pv_distill_max_entries()
 
 
+def _distill_args(lead, teacher_ids, teacher_logits, labels, temperature):
+    if teacher_logits.dim() != len(lead) + 1 or teacher_logits.shape[:-1] != lead or teacher_logits.shape[-1] < 1:
+        raise ValueError("teacher_logits has shape %s, expected %s" % (tuple(teacher_logits.shape), tuple(lead) + ("K",)))
+    if teacher_logits.shape[-1] > DISTILL_MAX:
+        raise ValueError("%d teacher entries a row, at most %d are taken" % (teacher_logits.shape[-1], DISTILL_MAX))
+    if teacher_logits.dtype not in _ROW_DTYPES:
+        raise ValueError("teacher_logits must be float32, bfloat16 or float16 (got %s)" % teacher_logits.dtype)
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("teacher_logits is a constant of this loss: detach it")
+    _check_temp(temperature)
+    return (_index("teacher_ids", teacher_ids, teacher_logits.shape), teacher_logits.detach().contiguous(),
+            None if labels is None else _index("labels", labels, lead))
+
+
 def distill_topk(logits, teacher_ids, teacher_logits, labels=None, ignore_index=None, temperature=1.0, weight=1.0,
                  avg_type="seq"):
     """Distillation of `logits` [..., V] from a teacher's top logits: teacher_ids (int) / teacher_logits [..., K], K <= 256.
@@ -2911,26 +2925,14 @@ def distill_topk(logits, teacher_ids, teacher_logits, labels=None, ignore_index=
     names no word makes the loss NaN.  A coefficient belongs into `weight`: an upstream gradient other than 1 costs another
     pass over the rows."""
     _check_rows(logits)
-    lead = logits.shape[:-1]
-    if teacher_logits.dim() != logits.dim() or teacher_logits.shape[:-1] != lead or teacher_logits.shape[-1] < 1:
-        raise ValueError("teacher_logits has shape %s, expected %s" % (tuple(teacher_logits.shape), tuple(lead) + ("K",)))
-    if teacher_logits.shape[-1] > DISTILL_MAX:
-        raise ValueError("%d teacher entries a row, at most %d are taken" % (teacher_logits.shape[-1], DISTILL_MAX))
-    if teacher_logits.dtype not in _ROW_DTYPES:
-        raise ValueError("teacher_logits must be float32, bfloat16 or float16 (got %s)" % teacher_logits.dtype)
-    if teacher_logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError("teacher_logits is a constant of this loss: detach it")
-    teacher_ids = _index("teacher_ids", teacher_ids, teacher_logits.shape)
-    if labels is not None:
-        labels = _index("labels", labels, lead)
-    _check_temp(temperature)
+    ids, tl, labels = _distill_args(logits.shape[:-1], teacher_ids, teacher_logits, labels, temperature)
     w, word = _avg(avg_type, weight, logits.shape[0] if logits.dim() > 1 else 1)
-    _same_device(logits, teacher_ids, teacher_logits, labels)
-    if teacher_ids.numel() == 0:
+    _same_device(logits, ids, tl, labels)
+    if ids.numel() == 0:
         return logits.to(torch.float32).sum() * 0.0
     want = logits.requires_grad and torch.is_grad_enabled()
-    return DistillTopK.apply(logits, teacher_ids, teacher_logits.detach().contiguous(), labels,
-                             _NO_INDEX if ignore_index is None else int(ignore_index), 1.0 / float(temperature), w, word, want)
+    return DistillTopK.apply(logits, ids, tl, labels, _NO_INDEX if ignore_index is None else int(ignore_index),
+                             1.0 / float(temperature), w, word, want)
 
 
 class VocabPolicyLoss(torch.autograd.Function):
@@ -2945,7 +2947,7 @@ class VocabPolicyLoss(torch.autograd.Function):
         d = _one_pass_grad(logits, want_grad)
         _launch(dev, "pv_policy_rows_fwd", *_row_args(x), _p(tokens), ignore, inv_temp, _p(old), _p(ref), _p(adv),
                 int(adv.numel() == T), lo, hi, kl, ent, weight, word, _p(loss), _p(stats), save if want_grad else None,
-                _p(d), save + 16 * T)
+                _p(d), 0, None, save + 16 * T)
         if want_grad:
             ctx.save_for_backward(x, tokens, buf)
             ctx.grad = d
@@ -3043,6 +3045,150 @@ def policy_loss(logp, tokens, old_logp, advantages, ref_logp=None, ignore_index=
     want = logp.requires_grad and torch.is_grad_enabled()
     return PolicyLoss.apply(logp, tokens, old, ref, adv, _NO_INDEX if ignore_index is None else int(ignore_index), lo, hi, kl, w,
                             word, want)
+
+
+class ProjectedLoss(torch.autograd.Function):
+    """A loss over vocabulary rows behind the projection hid W^T + b, with the gradients of all three: the logits live in fp32
+    between two kernels, their gradient in bf16 as the operand of the two products that follow (the projection's own operands
+    are bf16 too).  Rows that are dead by `labels` go last and are not multiplied.
+    run(row arguments, gradient or None, its row length, order of the rows or None) -> (loss, further outputs): the C call."""
+
+    @staticmethod
+    def forward(ctx, hid, weight, bias, labels, ignore, run, want_grad):
+        B, L, H = hid.shape
+        dev, V, T = hid.device, weight.shape[0], B * L
+        Hp, Vp, Tp = round_up(H, 64), round_up(V, 64), round_up(T, 64)
+        h_bf = torch.empty((Tp, Hp), dtype=BF16, device=dev)
+        cast_pack(hid, B, L, L, H, hid.stride(0), hid.stride(1), hid.stride(2), Hp, out=h_bf)
+        w_bf = pack_matrix(weight, Hp)
+        d = perm = live = None
+        if want_grad:
+            d = torch.empty((Tp, Vp), dtype=BF16, device=dev)
+            if labels is not None:
+                perm = torch.empty(T, dtype=torch.int64, device=dev)
+                live = torch.empty(1, dtype=torch.int32, device=dev)
+                _launch(dev, "pv_vocab_compact", _p(labels), T, ignore, _p(perm), _p(live))
+                all_h, h_bf = h_bf, torch.empty((Tp, Hp), dtype=BF16, device=dev)
+                _launch(dev, "pv_vocab_gather", _p(all_h), Hp, _p(labels), _p(perm), T, Hp, _p(h_bf), Hp,
+                        _p(torch.empty(T, dtype=torch.int64, device=dev)))
+            if Tp > T:                             # the token extent of the weight gradient's product
+                d[T:].zero_()
+                h_bf[T:].zero_()
+        logits = gemm_nt(h_bf, Hp, w_bf, Hp, T, V, Hp, bias=bias.contiguous(),
+                         out=torch.empty((T, Vp), dtype=torch.float32, device=dev), m_live=live)
+        out = run((_p(logits), _ROW_DTYPES[torch.float32], B, L, L * Vp, Vp, V), d, Vp, perm)
+        ctx.save_for_backward(h_bf, w_bf, d, perm, live)
+        ctx.dims = (B, L, H, V)
+        ctx.mark_non_differentiable(*out[1:])
+        return out
+
+    @staticmethod
+    @_one_derivative
+    def backward(ctx, g, *_):
+        h_bf, w_bf, d, perm, live = ctx.saved_tensors
+        B, L, H, V = ctx.dims
+        dev, T, (Tp, Vp), Hp = d.device, B * L, d.shape, h_bf.shape[1]
+        need_h, need_w, need_b = ctx.needs_input_grad[:3]
+        dh = dw = db = None
+        if need_h:
+            dh = torch.empty(round_up(T * H, 4), dtype=torch.float32, device=dev)
+            wt = transpose_to_bf16(w_bf, V, H, Hp, Vp)
+            if perm is None:
+                gemm_nt(d, Vp, wt, Vp, T, H, Vp, out=dh[:T * H].view(T, H))
+            else:
+                part = gemm_nt(d, Vp, wt, Vp, T, H, Vp, m_live=live)
+                _launch(dev, "pv_scatter_rows_f32", _p(part), H, _p(perm), _p(live), T, H, _p(dh), H)
+            _launch(dev, "pv_scale_by_f32", _p(dh), dh.numel(), _p(g))
+            dh = dh[:T * H].view(B, L, H)
+        if need_w:
+            dw = torch.empty(round_up(V * H, 4), dtype=torch.float32, device=dev)
+            splits = C.c_int(1)
+            _lib.call("pv_gemm_splitk_plan", V, H, Tp, 2 * torch.cuda.get_device_properties(dev).multi_processor_count,
+                      C.byref(splits))
+            ws = torch.empty(_lib.load().pv_gemm_splitk_ws_bytes(V, H, splits.value) if splits.value > 1 else 0,
+                             dtype=torch.uint8, device=dev)
+            _launch(dev, "pv_gemm_bf16_tn_splitk", _p(d), Vp, _p(h_bf), Hp, V, H, Tp, max(1, splits.value),
+                    _p(ws) if splits.value > 1 else None, _p(dw), H, 0)
+            _launch(dev, "pv_scale_by_f32", _p(dw), dw.numel(), _p(g))
+            dw = dw[:V * H].view(V, H)
+        if need_b:
+            db = torch.empty(V, dtype=torch.float32, device=dev)
+            ws = torch.empty(_lib.load().pv_colsum_scaled_ws_bytes(V), dtype=torch.uint8, device=dev)
+            _launch(dev, "pv_colsum_scaled_bf16", _p(d), Vp, T, V, _p(g), _p(db), _p(ws))
+        return dh, dw, db, None, None, None, None
+
+
+def projection_fits(vocab_size):
+    """Whether the losses behind a projection take a vocabulary (a row of fp32 logits is held on chip)."""
+    return bool(_lib.load().pv_vocab_rows_one_pass(_ROW_DTYPES[torch.float32], int(vocab_size)))
+
+
+def _projection(hid, weight, bias):
+    """Checks -> the leading shape [B, L]."""
+    if hid.dim() != 3 or hid.dtype != torch.float32:
+        raise ValueError("hid must be float32 [B, L, H] (got %s %s)" % (hid.dtype, tuple(hid.shape)))
+    V = weight.shape[0]
+    if weight.shape != (V, hid.shape[2]) or bias.shape != (V,) or weight.dtype != torch.float32 or bias.dtype != torch.float32:
+        raise ValueError("a float32 projection [V, %d] with bias [V] is needed (got %s and %s)"
+                         % (hid.shape[2], tuple(weight.shape), tuple(bias.shape)))
+    if not projection_fits(V):
+        raise ValueError("a vocabulary of %d words does not fit here: take the loss over materialised rows" % V)
+    return hid.shape[:2]
+
+
+def _projected(hid, weight, bias, labels, ignore, run):
+    want = torch.is_grad_enabled() and (hid.requires_grad or weight.requires_grad or bias.requires_grad)
+    with torch.cuda.device(hid.device):
+        return ProjectedLoss.apply(hid, weight, bias, labels, ignore, run, want)
+
+
+def projected_distill_topk(hid, proj_weight, proj_bias, teacher_ids, teacher_logits, labels=None, ignore_index=None, inv_temp=1.0,
+                           temperature=1.0, weight=1.0, avg_type="seq"):
+    """distill_topk of the logits (hid W^T + b) * inv_temp, hid [B, L, H] fp32, W [V, H], differentiable in hid, W and b.  The
+    operands of the products are bf16 and so is the logits' gradient between them; everything else is fp32."""
+    shape = _projection(hid, proj_weight, proj_bias)
+    ids, tl, labels = _distill_args(shape, teacher_ids, teacher_logits, labels, temperature)
+    _check_temp(inv_temp)
+    w, word = _avg(avg_type, weight, shape[0])
+    dev = _same_device(hid, proj_weight, proj_bias, ids, tl, labels)
+    if ids.numel() == 0:
+        return hid.sum() * 0.0
+    ignore, K, T = _NO_INDEX if ignore_index is None else int(ignore_index), ids.shape[-1], shape[0] * shape[1]
+
+    def run(rows, d, ld, perm):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        buf, save = _bytes(16 * T + _ws_bytes(T) + 4 * T * K, dev)
+        ws = save + 16 * T
+        _launch(dev, "pv_distill_rows_fwd", *rows, _p(labels), ignore, inv_temp / temperature, 1.0 / temperature, _p(ids), _p(tl),
+                _ROW_DTYPES[tl.dtype], K, w, word, _p(loss), save, ws + _ws_bytes(T), _p(d), 0 if d is None else ld, _p(perm),
+                ws)
+        return (loss,)
+    return _projected(hid, proj_weight, proj_bias, labels, ignore, run)[0]
+
+
+def projected_policy_loss(hid, proj_weight, proj_bias, tokens, old_logp, advantages, ref_logp=None, ignore_index=None, inv_temp=1.0,
+                          clip=0.2, clip_high=None, kl_coef=0.0, ent_coef=0.0, weight=1.0, avg_type="word"):
+    """vocab_policy_loss of the logits (hid W^T + b), see projected_distill_topk; for a loss without an entropy term policy_loss
+    behind the fused vocabulary projection does without the logits altogether."""
+    shape = _projection(hid, proj_weight, proj_bias)
+    tokens = _index("tokens", tokens, shape)
+    old, ref, adv, lo, hi, kl = _policy_args(shape, old_logp, advantages, ref_logp, clip, clip_high, kl_coef)
+    _check_temp(inv_temp)
+    w, word = _avg(avg_type, weight, shape[0])
+    dev = _same_device(hid, proj_weight, proj_bias, tokens, old, adv, ref)
+    T = tokens.numel()
+    if T == 0:
+        return hid.sum() * 0.0, torch.zeros(4, dtype=torch.float32, device=dev)
+    ignore = _NO_INDEX if ignore_index is None else int(ignore_index)
+
+    def run(rows, d, ld, perm):
+        loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
+        buf, save = _bytes(16 * T + _ws_bytes(T), dev)
+        _launch(dev, "pv_policy_rows_fwd", *rows, _p(tokens), ignore, float(inv_temp), _p(old), _p(ref), _p(adv),
+                int(adv.numel() == T), lo, hi, kl, float(ent_coef), w, word, _p(loss), _p(stats), save, _p(d),
+                0 if d is None else ld, _p(perm), save + 16 * T)
+        return loss, stats
+    return _projected(hid, proj_weight, proj_bias, tokens, ignore, run)
 
 
 class PreferenceLoss(torch.autograd.Function):

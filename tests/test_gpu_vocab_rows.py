@@ -731,6 +731,108 @@ def test_refusals_on_the_device(dev):
 # together, behind the decoder
 # ------------------------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("shape", [(1, 1, 16, 2), (2, 3, 48, 7), (3, 5, 64, 1003), (4, 33, 128, 777), (2, 9, 512, 20004), (1, 3, 32, 65001)])
+@pytest.mark.parametrize("kind", ["distill", "policy"])
+def test_losses_behind_a_projection(dev, shape, kind):
+    """Against 64 bits on the operands as the products see them (bf16).  A logit sums H products in fp32 (off by less than
+    H u of their magnitudes); the logits' gradient is rounded to bf16 once (2^-8 of each element), and the products of it sum
+    V or B L terms in fp32 (their count times u of the magnitudes, 4e-3 at most here, far less in fact: 1e-4 is granted)."""
+    from pevae_amd import ops
+    B, L, H, V = shape
+    gen = torch.Generator(device=dev).manual_seed(200 + V)
+    hid = (torch.randn(L, B, H, generator=gen, device=dev) * 0.5).transpose(0, 1).requires_grad_()        # time major
+    w = (torch.randn(V, H, generator=gen, device=dev) * 0.2).requires_grad_()
+    b = torch.randn(V, generator=gen, device=dev).requires_grad_()
+    y = labels_of((B, L), V, dev, 201, 0.3)
+    live = y != -7
+    h64, w64 = hid.detach().bfloat16().double(), w.detach().bfloat16().double()
+    z = h64 @ w64.t() + b.detach().double()
+    zerr = H * 2.0 ** -24 * (h64.abs() @ w64.abs().t() + b.detach().abs().double()).max() / EXP             # in units of EXP
+    c, tau = 1.0 / 0.8, 1.5
+    if kind == "distill":
+        K = min(V, 6)
+        t = (make((B, L, V), torch.float32, dev, 202) + 0.5 * z.float()).topk(K, -1)
+        n = max(int(live.sum()), 1)
+        loss = ops.projected_distill_topk(hid, w, b, t.indices, t.values, y, -7, c, tau, 2.0, "word")
+        p, lq = softmax64(z, c / tau)
+        q, lt = softmax64(t.values, 1.0 / tau)
+        on = live.double() * 2.0 / n
+        rows = (q * (lt - lq.gather(-1, t.indices))).sum(-1)
+        want, mag = tau * tau * (on * rows).sum(), tau * tau * (on * ((q * (lt.abs() + lq.gather(-1, t.indices).abs())).sum(-1) + 1)).sum()
+        target = torch.zeros_like(p).scatter_add_(-1, t.indices, q)
+        dz, dmag = (on * tau * c)[..., None] * (p - target), (on * tau * c)[..., None] * (p + target)
+        outs = (loss,)
+    else:
+        p, lq = softmax64(z, c)
+        Hh = -plogp(p, lq).sum(-1)
+        lp = lq.gather(-1, y.clamp(min=0)[..., None])[..., 0]
+        old, ref, adv = policy_inputs(lp, dev, 203)
+        loss, stats = ops.projected_policy_loss(hid, w, b, y, old, adv, ref, -7, c, 0.2, 0.28, 0.1, 0.05, 2.0, "seq")
+        pg, k3, cut, slope, smag = policy64(lp, old.double(), ref.double(), adv.double(), live, 0.8, 1.28, 0.1)
+        on = live.double() * 2.0 / B
+        want = (2.0 / B) * (pg + 0.1 * k3).sum() - 0.05 * (on * Hh).sum()
+        mag = (2.0 / B) * (pg.abs() + 3 * smag + 0.1 * k3).sum() + 0.05 * (on * (1 + Hh)).sum()
+        yl = torch.where(live, y, torch.full_like(y, -1))
+        dz, _ = rows_grad64(p, lq, Hh, yl, (2.0 / B) * slope, -0.05 * on, c)
+        _, dmag = rows_grad64(p, lq, Hh, yl, (2.0 / B) * 3 * smag, -0.05 * on, c)
+        outs = (loss, stats)
+        assert not stats.requires_grad
+    close(loss, want, (1 + zerr) * mag + 1e-30, "loss")
+    err = (2.0 ** -8 + 1e-4) * dz.abs() + (EXP * (1 + zerr) + 1e-4) * dmag
+    d2, e2, h2 = dz.reshape(B * L, V), err.reshape(B * L, V), h64.reshape(B * L, H)
+    for up in (None, torch.tensor(-2.5, device=dev), None):
+        k = 1.0 if up is None else -2.5
+        gh, gw, gb = torch.autograd.grad(loss, [hid, w, b], up, retain_graph=True)
+        for got, exact, tol, name in ((gh.reshape(B * L, H), d2 @ w64, e2 @ w64.abs(), "hid"), (gw, d2.t() @ h2, e2.t() @ h2.abs(), "weight"),
+                                      (gb, d2.sum(0), e2.sum(0), "bias")):
+            over = (got.double() - k * exact).abs() / (abs(k) * tol + 1e-30)
+            assert float(over.max()) <= 1.0, "%s: %.3g of the tolerance" % (name, float(over.max()))
+    with torch.no_grad():
+        again = ops.projected_distill_topk(hid, w, b, t.indices, t.values, y, -7, c, tau, 2.0, "word") if kind == "distill" else \
+            ops.projected_policy_loss(hid, w, b, y, old, adv, ref, -7, c, 0.2, 0.28, 0.1, 0.05, 2.0, "seq")[0]
+    close(again, want, (1 + zerr) * mag + 1e-30, "loss alone")
+    only, = torch.autograd.grad(ops.projected_distill_topk(hid.detach(), w.detach(), b, t.indices, t.values, y, -7, c, tau, 2.0, "word")
+                                if kind == "distill" else
+                                ops.projected_policy_loss(hid.detach(), w.detach(), b, y, old, adv, ref, -7, c, 0.2, 0.28, 0.1, 0.05,
+                                                          2.0, "seq")[0], b)
+    assert torch.equal(only, gb)
+
+
+def test_losses_behind_a_projection_captured(dev):
+    """A graph of forward and backward, replayed with eager work and changed inputs between."""
+    from pevae_amd import ops
+    B, L, H, V = 5, 7, 64, 2003
+    y = labels_of((B, L), V, dev, 210)
+    ids = torch.arange(9, device=dev).expand(B, L, 9).contiguous()
+    t = make((B, L, 9), torch.float32, dev, 211)
+    old, adv = make((B, L), torch.float32, dev, 212) - 8, make((B,), torch.float32, dev, 213)
+    params = [make(s, torch.float32, dev, k, 0.3) for k, s in ((214, (B, L, H)), (215, (V, H)), (216, (V,)))]
+
+    def step(xs):
+        a = ops.projected_distill_topk(*xs, ids, t, y, -7)
+        b = ops.projected_policy_loss(*xs, y, old, adv, old, -7, kl_coef=0.1, ent_coef=0.01)[0]
+        return [a.detach(), b.detach()] + [g for x in (a, b) for g in torch.autograd.grad(x, xs)]
+
+    held = [x.clone().requires_grad_() for x in params]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(held)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(held)
+    for turn in range(3):
+        with torch.no_grad():
+            for x, v in zip(held, params):
+                x.copy_(v * (1.0 + 0.1 * turn))
+        want = step([(v * (1.0 + 0.1 * turn)).requires_grad_() for v in params])
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
 def test_decoder_learns_from_a_teacher_and_from_judgments(dev):
     """A decoder scores sampled answers, distils a teacher, takes a policy and a preference step: through its DeferredLogProbs
     (the fused projection) and through its dense rows, both against the losses of the dense rows in 64 bits.  The projection
@@ -759,6 +861,7 @@ def test_decoder_learns_from_a_teacher_and_from_judgments(dev):
     policy = criterions.ClippedPolicyLoss(0, None, kl_coef=0.1)
     prefer = criterions.PreferenceLoss(0, None, beta=0.5)
     distill = criterions.TopKDistill(0, None, temperature=2.0)
+    explore = criterions.ClippedPolicyLoss(0, None, kl_coef=0.1, ent_coef=0.1)
     h = B // 2
     half = [outs_slice for outs_slice in (slice(0, h), slice(h, B))]
 
@@ -767,12 +870,13 @@ def test_decoder_learns_from_a_teacher_and_from_judgments(dev):
             return dec(h, ids[s], h0[:, s].contiguous(), mode=D.TEACH_FORCE)[0]
         return [distill(view(outs()), y, teacher.indices, teacher.values),
                 policy(view(outs()), y, old, adv, ref)[0],
-                prefer(view(part(half[0])), y[half[0]], view(part(half[1])), y[half[1]], ref[half[0]], ref[half[1]])[0]]
+                prefer(view(part(half[0])), y[half[0]], view(part(half[1])), y[half[1]], ref[half[0]], ref[half[1]])[0],
+                explore(view(outs()), y, old, adv, ref)[0]]
 
     roads = []
     for view in (lambda o: o, lambda o: o.materialize()):
         got = []
-        for k in range(3):
+        for k in range(4):
             dec.zero_grad()
             loss = losses(view)[k]
             loss.backward()
@@ -786,8 +890,10 @@ def test_decoder_learns_from_a_teacher_and_from_judgments(dev):
     want1 = (pg + 0.1 * k3).sum() / int(live.sum())
     dl = torch.where(live, lp64 - ref.double(), torch.zeros_like(lp64)).sum(1)
     want2 = -torch.nn.functional.logsigmoid(0.5 * (dl[:h] - dl[h:])).mean()
+    ent = -plogp(torch.exp(x), x).sum(-1)
+    want3 = want1 - 0.1 * torch.where(live, ent, torch.zeros_like(ent)).sum() / int(live.sum())
     for road in roads:
-        for (loss, gw, gb), want in zip(road, (want0, want1, want2)):
+        for (loss, gw, gb), want in zip(road, (want0, want1, want2, want3)):
             assert abs(loss - float(want)) <= 2e-3 * (1 + abs(float(want)))
             assert float(gw.abs().max()) > 0 and bool(torch.isfinite(gw).all())
     for a, b in zip(*roads):

@@ -26,7 +26,9 @@ def test_valid_arguments_on_the_cpu_raise_for_the_device():
                  lambda: ops.vocab_policy_loss(rows(), ids(2, 3), f(2, 3), f(2)),
                  lambda: ops.policy_loss(f(2, 3), ids(2, 3), f(2, 3), f(2, 3)),
                  lambda: ops.preference_loss(f(2, 3), ids(2, 3), f(2, 4), ids(2, 4)),
-                 lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(L=4), ids(2, 4))):
+                 lambda: ops.vocab_preference_loss(rows(), ids(2, 3), rows(L=4), ids(2, 4)),
+                 lambda: ops.projected_distill_topk(f(2, 3, 8), f(5, 8), f(5), ids(2, 3, 2), f(2, 3, 2)),
+                 lambda: ops.projected_policy_loss(f(2, 3, 8), f(5, 8), f(5), ids(2, 3), f(2, 3), f(2))):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
 
@@ -69,6 +71,22 @@ def test_bad_arguments_raise_value_errors(call):
         call()
 
 
+@pytest.mark.parametrize("call", [
+    lambda h, w, b: ops.projected_distill_topk(h[0], w, b, ids(2, 3, 2), f(2, 3, 2)),
+    lambda h, w, b: ops.projected_distill_topk(h.double(), w, b, ids(2, 3, 2), f(2, 3, 2)),
+    lambda h, w, b: ops.projected_distill_topk(h, w[:, :4], b, ids(2, 3, 2), f(2, 3, 2)),
+    lambda h, w, b: ops.projected_distill_topk(h, w, b[:4], ids(2, 3, 2), f(2, 3, 2)),
+    lambda h, w, b: ops.projected_distill_topk(h, w, b, ids(2, 3, 2), f(2, 4, 2)),
+    lambda h, w, b: ops.projected_distill_topk(h, w, b, ids(2, 3, 2), f(2, 3, 2), inv_temp=0.0),
+    lambda h, w, b: ops.projected_policy_loss(h, w, b, ids(2, 3), f(2, 3), f(3)),
+    lambda h, w, b: ops.projected_policy_loss(h, w, b, ids(2, 3), f(2, 3), f(2), kl_coef=0.5),
+    lambda h, w, b: ops.projected_distill_topk(f(1, 1, 2), f(81924, 2), f(81924), ids(1, 1, 2), f(1, 1, 2)),         # does not fit
+])
+def test_bad_projections_raise_value_errors(call):
+    with pytest.raises(ValueError):
+        call(f(2, 3, 8), f(5, 8), f(5))
+
+
 def test_criterions_refuse_unknown_averages():
     for cls in (criterions.TopKDistill, criterions.ClippedPolicyLoss, criterions.PreferenceLoss):
         with pytest.raises(NotImplementedError):
@@ -89,14 +107,19 @@ def test_entry_points_refuse_on_the_host():
         assert b"pv_token_logp_fwd" in lib.pv_last_error()
     assert logp(n0=1 << 16, n1=1 << 15) == -3
     assert logp(V=(1 << 24) + 1) == -3
-    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, None, p, None) == -3
-    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, None, p, None) == -1
-    assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, None, p, None) == -1
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, None, 0, None, p, None) == -3
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, None, 0, None, p, None) == -1
+    assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, None, 0, None, p, None) == -1
     assert lib.pv_policy_tokens_fwd(p, p, 0, 0, 4, p, None, p, 0, 0.8, 1.2, 0.0, 1.0, 0, p, p, p, p, None) == -1
     assert lib.pv_preference_fwd(None, None, None, 3, p, None, p, 3, 2, 0, 0.1, 0.0, 1.0, p, p, p, p, None) == -1
     assert lib.pv_vocab_rows_one_pass(0, 81923) == 1 and lib.pv_vocab_rows_one_pass(0, 81924) == 0     # 20 480 pieces of 16 bytes
     assert lib.pv_vocab_rows_one_pass(1, 163847) == 1 and lib.pv_vocab_rows_one_pass(2, 163848) == 0
-    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 81924, 81924, None, 0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, p, None) == -1
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 81924, 81924, None, 0, 1.0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, 0, None, p, None) == -1
+    for dtype, ld in ((0, 4), (0, 70), (1, 64)):                # shorter than a row, too long, not fp32
+        assert lib.pv_distill_rows_fwd(p, dtype, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, ld, None, p, None) == -1
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 0.0, p, p, 0, 4, 1.0, 0, p, p, p, None, 0, None, p, None) == -1
+    assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 0, 4, 1.0, 0, p, p, p, p, 0, p, p, None) == -1
+    assert lib.pv_colsum_scaled_bf16(p, 7, 4, 7, p, p, p, None) == -1 and lib.pv_scale_by_f32(p, 6, p, None) == -1
     assert lib.pv_preference_rows_fwd(p, 0, 2, 3, 15, 5, 5, p, None, p, 0, 0, 15, 5, 5, p, None, 0, 1.0, 0.1, 0.0, 1.0, p, p, p, p, p, p,
                                       None) == -1
     assert lib.pv_preference_rows_bwd(p, 0, 2, 3, 15, 5, 5, p, 0, 1.0, None, p, 1.0, p, p, None) == -1
