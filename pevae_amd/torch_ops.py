@@ -73,3 +73,16 @@ def _(emb_weight, w_ih, w_hh, b_ih, b_hh, proj_weight, proj_bias, h0, length, so
     B, H = h0.shape
     return (h0.new_empty((B, length), dtype=torch.int64), h0.new_empty((B, length), dtype=torch.float32),
             h0.new_empty((B, H), dtype=torch.float32))
+
+
+@torch.library.custom_op(NAMESPACE + "::token_logprobs", mutates_args=())
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int, inv_temp: float) -> torch.Tensor:
+    """pv_token_logp_fwd: log-probability of each row's token (0 where it is ignore_index), no [T, V] tensor beside the logits;
+    what a policy or preference loss asks of the old policy and of a reference model.  No gradient."""
+    with torch.no_grad():
+        return ops.token_logprobs(logits, tokens, ignore_index, inv_temp)
+
+
+@token_logprobs.register_fake
+def _(logits, tokens, ignore_index, inv_temp):
+    return logits.new_empty(tokens.shape, dtype=torch.float32)

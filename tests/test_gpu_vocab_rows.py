@@ -710,6 +710,14 @@ def test_captured_and_replayed(dev):
             assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k])), (turn, k)
 
 
+def test_registered_operator(dev):
+    import pevae_amd.torch_ops  # noqa: F401
+    from pevae_amd import ops
+    z = make((3, 4, 501), torch.float16, dev, 120)
+    y = labels_of((3, 4), 501, dev, 121)
+    assert torch.equal(torch.ops.pevae_amd.token_logprobs(z, y, -7, 0.9), ops.token_logprobs(z, y, -7, 0.9))
+
+
 def test_refusals_on_the_device(dev):
     """An input changed in place after the forward pass, and a second derivative, are refused."""
     from pevae_amd import ops

@@ -71,6 +71,15 @@ def test_bad_arguments_raise_value_errors(call):
         call()
 
 
+def test_registered_operator_has_a_fake_shape():
+    import pevae_amd.torch_ops  # noqa: F401
+    lp = torch.ops.pevae_amd.token_logprobs(torch.empty(4, 6, 500, device="meta", dtype=torch.bfloat16),
+                                            torch.empty(4, 6, device="meta", dtype=torch.int64), 0, 1.0)
+    assert lp.shape == (4, 6) and lp.dtype == torch.float32
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        torch.ops.pevae_amd.token_logprobs(rows(), ids(2, 3), 0, 1.0)
+
+
 @pytest.mark.parametrize("call", [
     lambda h, w, b: ops.projected_distill_topk(h[0], w, b, ids(2, 3, 2), f(2, 3, 2)),
     lambda h, w, b: ops.projected_distill_topk(h.double(), w, b, ids(2, 3, 2), f(2, 3, 2)),
