@@ -530,7 +530,8 @@ int pv_dropout_pack_bf16(const float* src, int n0, int n1, int n1p, int C, long 
  * logits: [n0][n1] rows of V words, words contiguous, rows at any element stride (s0, s1) and any element address, dtype
  * PV_DTYPE_*; log-probabilities serve as logits.  inv_temp: 1 / temperature.  tokens / labels: int64 [n0 * n1]; rows whose
  * entry is `ignore` are dead: not read, zero in every output.  A live entry outside [0, V) makes its row's outputs NaN, and
- * so does a row without a finite logit.  Limits: 2^31 - 1 rows, 2^24 words (PV_ERR_LIMIT).
+ * so does a row without a finite logit.  Limits (PV_ERR_LIMIT): 2^26 - 1 rows, and fewer than 2^32 threads a launch, of which
+ * a row gets 64 (up to 8 KB), 128 (16 KB), 256 (32 KB), 512 (64 KB) or 1024; 2^24 words; 2^24 - 1 pairs.
  * Gradients (dlogits) are contiguous [n0 * n1][V] of the logits' type.  `save`: 4 floats a row, handed from the forward to
  * the backward call (NULL: no gradient wanted).  ws: pv_vocab_rows_ws_bytes(rows). */
 #define PV_DTYPE_F32 0
@@ -544,9 +545,12 @@ size_t pv_vocab_rows_ws_bytes(long rows);
  * perm (NULL: none) then says that row t of the logits and of the gradient is row perm[t] of everything else, a permutation
  * that puts the dead rows, whose logits need not be there, last (pv_vocab_compact).
  * pv_colsum_scaled_bf16: out[v] = *g * sum over T such rows, in a fixed order; ws: pv_colsum_scaled_ws_bytes(V).
+ * pv_gather_live_rows_bf16: the operand's rows in that order, out[t] = t < *count ? h[perm[t]] : 0 for `rows` contiguous rows of
+ * H bf16 words (H % 8 == 0, 16-byte aligned; perm is read for live rows only).
  * pv_scale_by_f32: x *= *g (n % 4 == 0, 16-byte aligned; no pass where *g is 1). */
 size_t pv_colsum_scaled_ws_bytes(int V);
 int pv_colsum_scaled_bf16(const void* P, long ld, long T, int V, const float* g, float* out, void* ws, void* stream);
+int pv_gather_live_rows_bf16(const void* h, const int64_t* perm, const int* count, long rows, int H, void* out, void* stream);
 int pv_scale_by_f32(float* x, long n, const float* g, void* stream);
 int pv_vocab_rows_one_pass(int dtype, int V);
 /* logp[t] = log_softmax(logits * inv_temp)[t][tokens[t]]; entropy[t] (NULL: not wanted) of the same distribution.  Backward
@@ -558,7 +562,8 @@ int pv_token_logp_bwd(const void* logits, int dtype, long n0, int n1, long s0, l
                       void* dlogits, void* stream);
 /* Clipped policy loss of sampled tokens, with r = exp(logp - old_logp) and d = ref_logp - logp:
  *   loss = scale * sum over live rows of [ -min(r A, clip(r, clip_lo, clip_hi) A) + kl_coef (e^d - 1 - d) - ent_coef H ]
- * scale = weight, or weight / (live rows, at least 1) with word != 0.  ref_logp NULL: no KL term.  adv: [n0 * n1] with
+ * scale = weight, or weight / (live rows, at least 1) with word != 0.  ref_logp NULL: no KL term; kl_coef 0 with ref_logp: the
+ * term is reported and does not enter.  adv: [n0 * n1] with
  * adv_per_token, else [n0].  stats[4]: means over live rows of the policy term, of the KL term, of "the clip decides" and of
  * H.  Backward: g = upstream gradient of the loss (device scalar). */
 int pv_policy_rows_fwd(const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, const int64_t* tokens,

@@ -157,6 +157,7 @@ SIGNATURES = {
     "pv_distill_rows_fwd": (i32, _ROWS + [vp, i64, f32, f32, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, lng, vp, vp, vp]),
     "pv_colsum_scaled_ws_bytes": (sz, [i32]),
     "pv_colsum_scaled_bf16": (i32, [vp, lng, lng, i32, vp, vp, vp, vp]),
+    "pv_gather_live_rows_bf16": (i32, [vp, vp, vp, lng, i32, vp, vp]),
     "pv_scale_by_f32": (i32, [vp, lng, vp, vp]),
     "pv_distill_rows_bwd": (i32, _ROWS + [f32, vp, i32, vp, vp, vp, i32, vp, vp]),
     "pv_policy_tokens_fwd": (i32, [vp, vp, i64, lng, i32, vp, vp, vp, i32, f32, f32, f32, f32, i32, vp, vp, vp, vp, vp]),

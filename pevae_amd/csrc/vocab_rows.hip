@@ -19,6 +19,8 @@ namespace {
 
 constexpr int kTeacherMax = 256;        // teacher entries a row: four a lane of one wave
 constexpr int kVocabMax = 1 << 24;      // indices of a row fit fp32 and int32 with room
+constexpr long kRowsMax = (1L << 26) - 1;     // a wave a row: fewer than 2^32 threads a launch
+constexpr long kPairsMax = (1L << 24) - 1;    // 256 threads a pair
 constexpr float kFloorX = -2.0e4f;      // 2^kFloorX is 0: keeps 0 * (-inf) out of the entropy terms
 constexpr float kDead = __builtin_inff();   // `m` of a row that is not computed (padding, empty teacher list)
 
@@ -264,7 +266,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy& h, float lp, flo
   if (h.ref_lp) {
     const float d = ref_lp - lp, em1 = expm1f(d);
     o.k3 = exp_minus_1_minus(d, em1);
-    o.dlp -= h.kl * em1;
+    if (h.kl != 0.f) o.dlp -= h.kl * em1;         // (em1 may be infinite)
   }
   return o;
 }
@@ -710,7 +712,8 @@ struct Result {
 __device__ __forceinline__ void write_result(const double (&v)[5], const Result& r) {
   const double n = v[4] > 1.0 ? v[4] : 1.0;
   const double scale = r.word ? r.weight / n : r.weight;
-  *r.loss = (float)(scale * (v[0] + (double)r.kl * v[1] - (double)r.ent * v[3]));
+  const double kl = r.kl != 0.f ? (double)r.kl * v[1] : 0.0;         // the term may be infinite where it only is reported
+  *r.loss = (float)(scale * (v[0] + kl - (double)r.ent * v[3]));
   if (r.stats)
     for (int i = 0; i < 4; ++i) r.stats[i] = (float)(v[i] / n);
   if (r.scale) *r.scale = (float)scale;
@@ -848,6 +851,17 @@ __global__ __launch_bounds__(256) void scale_by_kernel(float4* __restrict__ x, l
   }
 }
 
+// Live rows of a bf16 matrix to the front, zeros behind them up to Tp rows: they meet the zero rows of the gradient in the
+// weight gradient's product, and what stands in dead rows of the caller's, NaN included, must not.
+__global__ __launch_bounds__(256) void gather_live_kernel(const uint4* __restrict__ h, const int64_t* __restrict__ perm,
+                                                          const int* __restrict__ count, int pieces, long n, uint4* __restrict__ out) {
+  const int live = *count;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) {
+    const uint32_t row = (uint32_t)(i / pieces);
+    out[i] = (int)row < live ? h[perm[row] * pieces + (i - (long)row * pieces)] : uint4{0u, 0u, 0u, 0u};
+  }
+}
+
 // ---- policy loss from log-probabilities ------------------------------------------------------------------------------------
 // Latency bound: a few bytes a token.  One launch up to 4096 tokens, and one more that adds the workgroups' sums beyond.
 __global__ __launch_bounds__(1024) void policy_tokens_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels,
@@ -966,28 +980,34 @@ __global__ __launch_bounds__(256) void preference_bwd_kernel(const int64_t* __re
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
+inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
 int check_rows(const char* who, const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp) {
   PV_REQUIRE(logits && n0 > 0 && n1 > 0 && V > 0, "%s: null logits or an empty size", who);
   PV_REQUIRE(dtype == PV_DTYPE_F32 || dtype == PV_DTYPE_BF16 || dtype == PV_DTYPE_F16, "%s: unknown dtype %d", who, dtype);
   PV_REQUIRE(s0 >= 0 && s1 >= 0, "%s: negative stride", who);
   PV_REQUIRE(inv_temp > 0.f && inv_temp < __builtin_inff(), "%s: the inverse temperature must be positive and finite", who);
   PV_REQUIRE(((uintptr_t)logits & (dtype == PV_DTYPE_F32 ? 3 : 1)) == 0, "%s: logits not aligned to their elements", who);
-  if (V > kVocabMax || n0 * (long)n1 > 0x7fffffffL) {
-    pv_set_error("%s: %ld rows of %d words are beyond the limit (2^31 - 1 rows, 2^24 words)", who, n0 * (long)n1, V);
+  if (V > kVocabMax || n0 > kRowsMax || n0 * (long)n1 > kRowsMax) {
+    pv_set_error("%s: %ld x %d rows of %d words are beyond the limit (%ld rows, 2^24 words)", who, n0, n1, V, kRowsMax);
+    return PV_ERR_LIMIT;
+  }
+  // a launch has fewer than 2^32 threads; the ladders below give a row at most these
+  const int pieces = pieces_of(dtype, V);
+  const long threads = pieces <= 512 ? 64 : pieces <= 1024 ? 128 : pieces <= 2048 ? 256 : pieces <= 4096 ? 512 : 1024;
+  if (n0 * (long)n1 * threads >= 1L << 32) {
+    pv_set_error("%s: %ld rows of %d words are more than a launch has threads for", who, n0 * (long)n1, V);
     return PV_ERR_LIMIT;
   }
   return PV_OK;
 }
-int check_count(const char* who, long n) {
-  if (n <= 0x7fffffffL) return PV_OK;
-  pv_set_error("%s: %ld are beyond the limit of 2^31 - 1", who, n);
+int check_count(const char* who, long n, long limit) {
+  if (n <= limit) return PV_OK;
+  pv_set_error("%s: %ld are beyond the limit of %ld", who, n, limit);
   return PV_ERR_LIMIT;
 }
 Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, const int64_t* labels, int64_t ignore, float c) {
   return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore, nullptr};
 }
-
-inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
 
 // Threads a row of the pass that only reads: a wave for short rows (V = 5003, bf16, 20000 rows: 39 us, 256 threads 49), more
 // for longer ones (V = 20004, bf16, 12800 rows, half of them dead: 256 threads 49 us, 64 58, 1024 82; V = 64001, fp32, 3000 rows:
@@ -1249,6 +1269,17 @@ int pv_colsum_scaled_bf16(const void* P, long ld, long T, int V, const float* g,
   return PV_OK;
 }
 
+int pv_gather_live_rows_bf16(const void* h, const int64_t* perm, const int* count, long rows, int H, void* out, void* stream) {
+  PV_REQUIRE(h && perm && count && out && rows > 0 && rows <= 0x7fffffffL && H > 0, "pv_gather_live_rows_bf16: bad argument");
+  PV_REQUIRE(H % 8 == 0 && ((uintptr_t)h & 15) == 0 && ((uintptr_t)out & 15) == 0,
+             "pv_gather_live_rows_bf16: rows must be 16-byte aligned");
+  const long n = rows * (H / 8), want = (n + 255) / 256;
+  gather_live_kernel<<<dim3((unsigned)(want > 4096 ? 4096 : want)), dim3(256), 0, (hipStream_t)stream>>>(
+      (const uint4*)h, perm, count, H / 8, n, (uint4*)out);
+  PV_LAUNCH_CHECK("gather_live_kernel");
+  return PV_OK;
+}
+
 int pv_scale_by_f32(float* x, long n, const float* g, void* stream) {
   PV_REQUIRE(x && g && n >= 0 && n % 4 == 0 && ((uintptr_t)x & 15) == 0, "pv_scale_by_f32: n must be a multiple of 4, x 16-byte aligned");
   if (n == 0) return PV_OK;
@@ -1265,7 +1296,7 @@ int pv_policy_tokens_fwd(const float* logp, const int64_t* tokens, int64_t ignor
   PV_REQUIRE(clip_lo <= clip_hi, "pv_policy_tokens_fwd: the clip range is empty");
   hipStream_t st = (hipStream_t)stream;
   const long T = n0 * (long)n1;
-  if (check_count("pv_policy_tokens_fwd", T) != PV_OK) return PV_ERR_LIMIT;
+  if (check_count("pv_policy_tokens_fwd", n0 > 0x7fffffffL ? n0 : T, 0x7fffffffL) != PV_OK) return PV_ERR_LIMIT;
   const Policy h = {old_logp, ref_logp, adv, adv_per_token, clip_lo, clip_hi, kl_coef, 0.f};
   const Result r = {kl_coef, 0.f, weight, word, loss, stats, dlogp ? dlogp + T : nullptr};
   const long want = T <= 4096 ? 1 : (T + 1023) / 1024;
@@ -1293,7 +1324,7 @@ int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* la
                       float smoothing, float weight, float* loss, float* rewards, float* slope, void* ws, void* stream) {
   PV_REQUIRE(loss && rewards && slope && ws && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_fwd: bad argument");
   PV_REQUIRE((Lc == 0 || (logp_c && labels_c)) && (Lr == 0 || (logp_r && labels_r)), "pv_preference_fwd: null argument");
-  if (check_count("pv_preference_fwd", pairs) != PV_OK) return PV_ERR_LIMIT;
+  if (check_count("pv_preference_fwd", pairs, kPairsMax) != PV_OK) return PV_ERR_LIMIT;
   hipStream_t st = (hipStream_t)stream;
   float4* rowout = (float4*)ws;
   preference_kernel<<<dim3((unsigned)pairs), dim3(256), 0, st>>>(Answers{logp_c, ref_c, labels_c, Lc},
@@ -1337,7 +1368,7 @@ int pv_preference_bwd(const int64_t* labels_c, int Lc, const int64_t* labels_r, 
                       const float* slope, float weight, const float* g, float* dlogp_c, float* dlogp_r, void* stream) {
   PV_REQUIRE(slope && g && pairs > 0 && Lc >= 0 && Lr >= 0, "pv_preference_bwd: bad argument");
   PV_REQUIRE((Lc == 0 || (labels_c && dlogp_c)) && (Lr == 0 || (labels_r && dlogp_r)), "pv_preference_bwd: null argument");
-  if (check_count("pv_preference_bwd", pairs) != PV_OK) return PV_ERR_LIMIT;
+  if (check_count("pv_preference_bwd", pairs, kPairsMax) != PV_OK) return PV_ERR_LIMIT;
   preference_bwd_kernel<<<dim3((unsigned)pairs), dim3(256), 0, (hipStream_t)stream>>>(labels_c, Lc, dlogp_c, labels_r, Lr, dlogp_r,
                                                                                       ignore, slope, weight, g);
   PV_LAUNCH_CHECK("preference_bwd_kernel");

@@ -82,7 +82,7 @@ class DeferredLogProbs(object):
         """(nll_tok, targets in row order): per-token -log p[label] (0 where label == ignore_index) without the logits.
         sums_only: the caller only wants {sum, live count}; where the fused kernels run, the first result is then that pair
         already (third result True) and the per-token vector is never put back into the caller's row order."""
-        key = (labels.data_ptr(), labels._version, tuple(labels.shape), ignore_index)
+        key = (labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
         hit = self._nll_cache.get(key)
         if hit is not None:
             return hit + (False,)
@@ -116,7 +116,7 @@ class DeferredLogProbs(object):
         return res + (False,)
 
     def _sums(self, labels, ignore_index):
-        key = ("sums", labels.data_ptr(), labels._version, tuple(labels.shape), ignore_index)
+        key = ("sums", labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
         hit = self._nll_cache.get(key)
         if hit is None:
             out, tgt, is_sums = self.token_nll(labels, ignore_index, sums_only=SUMS_ONLY)
@@ -132,7 +132,7 @@ class DeferredLogProbs(object):
     def loss_head(self, labels, ignore_index):
         """(NLLEntropy avg_type 'seq', Perplexity) of these labels as device scalars, one launch for both (ops.NllHead);
         the two criterions of a step ask for one each."""
-        key = ("head", labels.data_ptr(), labels._version, tuple(labels.shape), ignore_index)
+        key = ("head", labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
         hit = self._nll_cache.get(key)
         if hit is None:
             hit = self._nll_cache[key] = ops.NllHead.apply(self._sums(labels, ignore_index), self.hid.shape[0])
@@ -141,7 +141,8 @@ class DeferredLogProbs(object):
     def token_logp(self, labels, ignore_index):
         """Log-probability of `labels` [B, L] (0 where label == ignore_index) without the logits, differentiable."""
         B, L, _ = self.hid.shape
-        nll = self.token_nll(labels, ignore_index)[0]
+        ops._same_device(self.hid, labels)
+        nll = self.token_nll(ops._index("labels", labels, (B, L)), ignore_index)[0]
         if self.hid_bf16 is not None or (self.drop is not None and self.layout is not None):     # rows t * Bpad + b
             return -nll.view(L, self.layout[2])[:, :B].t()
         return -nll.view(B, L)

@@ -2852,7 +2852,7 @@ def token_logprobs(logits, tokens, ignore_index=None, inv_temp=1.0, entropy=Fals
     """Log-probability of `tokens` [...] under softmax(logits [..., V] * inv_temp), fp32, and with `entropy` the entropy of
     every row as well -> logp or (logp, entropy), both differentiable in `logits` (float32 / bfloat16 / float16, any strides;
     log-probabilities serve as logits).  Rows whose token is `ignore_index` are not read: 0, with a zero gradient.  Any other
-    token outside [0, V) makes its row NaN."""
+    token outside [0, V) makes its log-probability and its row's gradient NaN."""
     _check_rows(logits)
     tokens = _index("tokens", tokens, logits.shape[:-1])
     _check_temp(inv_temp)
@@ -3069,11 +3069,11 @@ class ProjectedLoss(torch.autograd.Function):
                 live = torch.empty(1, dtype=torch.int32, device=dev)
                 _launch(dev, "pv_vocab_compact", _p(labels), T, ignore, _p(perm), _p(live))
                 all_h, h_bf = h_bf, torch.empty((Tp, Hp), dtype=BF16, device=dev)
-                _launch(dev, "pv_vocab_gather", _p(all_h), Hp, _p(labels), _p(perm), T, Hp, _p(h_bf), Hp,
-                        _p(torch.empty(T, dtype=torch.int64, device=dev)))
+                _launch(dev, "pv_gather_live_rows_bf16", _p(all_h), _p(perm), _p(live), Tp, Hp, _p(h_bf))
             if Tp > T:                             # the token extent of the weight gradient's product
                 d[T:].zero_()
-                h_bf[T:].zero_()
+                if perm is None:
+                    h_bf[T:].zero_()
         logits = gemm_nt(h_bf, Hp, w_bf, Hp, T, V, Hp, bias=bias.contiguous(),
                          out=torch.empty((T, Vp), dtype=torch.float32, device=dev), m_live=live)
         out = run((_p(logits), _ROW_DTYPES[torch.float32], B, L, L * Vp, Vp, V), d, Vp, perm)

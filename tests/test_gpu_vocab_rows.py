@@ -419,6 +419,23 @@ def test_policy_edges(dev):
         assert float(loss) == 0.0 and float(d.abs().max()) == 0.0
 
 
+def test_policy_reports_a_far_reference(dev):
+    """A KL coefficient of 0 with a reference model: the term is reported (exp(190) is beyond fp32) and does not enter."""
+    from pevae_amd import ops
+    z = make((2, 3, 50), torch.float32, dev, 44).requires_grad_()
+    y = labels_of((2, 3), 50, dev, 45, 0.0)
+    old = ops.token_logprobs(z, y).detach() - 0.1
+    ref, adv = old.clone(), torch.tensor([1.0, -0.5], device=dev)
+    ref[0, 1] += 190.0
+    lp = ops.token_logprobs(z, y)
+    for with_ref, without in ((ops.vocab_policy_loss(z, y, old, adv, ref), ops.vocab_policy_loss(z, y, old, adv)),
+                              (ops.policy_loss(lp, y, old, adv, ref), ops.policy_loss(lp, y, old, adv))):
+        assert float(with_ref[0]) == float(without[0]) and float(with_ref[1][1]) == float("inf")
+        a, = torch.autograd.grad(with_ref[0], z, retain_graph=True)
+        b, = torch.autograd.grad(without[0], z, retain_graph=True)
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------------------------------------
 # preference
 # ------------------------------------------------------------------------------------------------------------
@@ -804,6 +821,52 @@ def test_losses_behind_a_projection(dev, shape, kind):
                                 ops.projected_policy_loss(hid.detach(), w.detach(), b, y, old, adv, ref, -7, c, 0.2, 0.28, 0.1, 0.05,
                                                           2.0, "seq")[0], b)
     assert torch.equal(only, gb)
+
+
+@pytest.mark.parametrize("shape", [(3, 5, 64, 1003), (2, 64, 40, 301)])
+def test_dead_rows_behind_a_projection_hold_anything(dev, shape):
+    """NaN and infinities in the states of dead rows reach no result."""
+    from pevae_amd import ops
+    B, L, H, V = shape
+    y = labels_of((B, L), V, dev, 220, 0.4)
+    hid, w, b = (make(s, torch.float32, dev, k, 0.3) for k, s in ((221, (B, L, H)), (222, (V, H)), (223, (V,))))
+    t = make((B, L, V), torch.float32, dev, 224).topk(5, -1)
+    old, adv = make((B, L), torch.float32, dev, 225) - 6, make((B,), torch.float32, dev, 226)
+    dead = torch.nonzero((y == -7).view(-1))[:, 0]
+    assert dead.numel() >= 2
+
+    def step(h):
+        xs = [x.clone().requires_grad_() for x in (h, w, b)]
+        loss = ops.projected_distill_topk(*xs, t.indices, t.values, y, -7), \
+            ops.projected_policy_loss(*xs, y, old, adv, old, -7, kl_coef=0.1, ent_coef=0.01)[0]
+        return [x.detach() for x in loss] + [g for x in loss for g in torch.autograd.grad(x, xs)]
+
+    foul = hid.clone()
+    foul.view(B * L, H)[dead[::2]] = float("nan")
+    foul.view(B * L, H)[dead[1::2]] = float("inf")
+    for a, c in zip(step(hid), step(foul)):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, c)
+
+
+def test_labels_of_deferred_rows(dev):
+    """Labels of any integer type and stride (views of one storage among them), and their refusals."""
+    from pevae_amd.enc2dec import decoders as D
+    B, L, H, V = 2, 4, 64, 77
+    hid, w, b = (make(s, torch.float32, dev, k, 0.3) for k, s in ((230, (B, L, H)), (231, (V, H)), (232, (V,))))
+    wide = labels_of((B, 2 * L), V, dev, 233)
+    out = D.DeferredLogProbs(hid, w, b, 1.0)
+    want = torch.log_softmax(out.materialize().double(), -1)
+    for y in (wide[:, ::2], wide[:, :L], wide[:, L:], wide[:, :L].to(torch.int32), wide[:, :L].contiguous()):
+        lp = out.token_logp(y, -7)
+        y = y.long()
+        exact = torch.where(y != -7, want.gather(-1, y.clamp(min=0)[..., None])[..., 0], 0.0)
+        assert float((lp - exact).abs().max()) <= 2e-4
+    with pytest.raises(RuntimeError):
+        out.token_logp(wide[:, :L].cpu(), -7)
+    with pytest.raises(ValueError):
+        out.token_logp(wide, -7)
+    with pytest.raises(ValueError):
+        out.token_logp(wide[:, :L].float(), -7)
 
 
 def test_losses_behind_a_projection_captured(dev):

@@ -116,6 +116,12 @@ def test_entry_points_refuse_on_the_host():
         assert b"pv_token_logp_fwd" in lib.pv_last_error()
     assert logp(n0=1 << 16, n1=1 << 15) == -3
     assert logp(V=(1 << 24) + 1) == -3
+    assert logp(n0=1 << 13, n1=1 << 13) == -3 and logp(n0=1 << 62) == -3          # 2^26 rows; more than 64 bits count
+    assert logp(n0=1 << 22, n1=1, V=16389, s0=0) == -3                            # 2^22 rows of 1024 threads
+    assert lib.pv_preference_fwd(p, None, p, 3, p, None, p, 3, 1 << 24, 0, 0.1, 0.0, 1.0, p, p, p, p, None) == -3
+    assert lib.pv_preference_bwd(p, 3, p, 3, 1 << 24, 0, p, 1.0, p, p, p, None) == -3
+    assert lib.pv_gather_live_rows_bf16(p, p, p, 4, 12, p, None) == -1
+    assert lib.pv_gather_live_rows_bf16(C.c_void_p(8), p, p, 4, 16, p, None) == -1
     assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 0, 257, 1.0, 0, p, p, p, None, 0, None, p, None) == -3
     assert lib.pv_distill_rows_fwd(p, 0, 1, 4, 0, 5, 5, None, 0, 1.0, 1.0, p, p, 7, 4, 1.0, 0, p, p, p, None, 0, None, p, None) == -1
     assert lib.pv_policy_rows_fwd(p, 0, 1, 4, 0, 5, 5, p, 0, 1.0, p, None, p, 0, 1.2, 0.8, 0.0, 0.0, 1.0, 0, p, p, p, None, 0, None, p, None) == -1
