@@ -223,7 +223,7 @@ struct Distill {
   const int64_t* ids;        // [T][K]
   const void* t_logits;      // [T][K]
   int K, dtype;
-  float* psum;               // [T][K]: the teacher's probability of the entry's word, duplicates added up
+  float* psum;               // [T][K]: the teacher's probability of the entry's word, duplicates added up; -1: nothing to add
   float c, k;                // 1 / temperature of the loss and of the teacher, c * log2(e)
 };
 struct Scale {
@@ -271,31 +271,92 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy& h, float lp, flo
   return o;
 }
 
-__device__ __forceinline__ float load_teacher(const Distill& h, long i) {
-  if (h.dtype == PV_DTYPE_F32) return ((const float*)h.t_logits)[i];
-  const uint16_t v = ((const uint16_t*)h.t_logits)[i];
-  return h.dtype == PV_DTYPE_BF16 ? bf2f(v) : (float)__builtin_bit_cast(_Float16, v);
-}
-
 // The teacher's side of a row, by one wave: its softmax over the K entries (those of -inf do not count), the sum of
 // p (log p - c (z - zref)) over the entries, and for each entry the probability of its word (duplicate words added up).
 // empty: no entry counts.  bad: an entry that counts names a word outside the vocabulary.
+// Its loads are asked for before the row's own (behind them they would arrive last, and the words' logits a latency later), and
+// the words' logits are kept for the end of the row: V = 5003, bf16, K = 64, 20000 rows: 102 us, 122 without either and with a sum
+// over the list for every entry of it.
 struct Teacher {
   float acc, zref;
   bool empty, bad;
 };
 struct TeacherList {         // of a row, in shared memory
-  int id[kTeacherMax];       // -1: no word of the vocabulary
-  float p[kTeacherMax], psum[kTeacherMax];
+  int id[kTeacherMax];       // -1: no word of the vocabulary, or nothing to add to it
+  float p[kTeacherMax], z[kTeacherMax], psum[kTeacherMax];     // of an entry: probability, its word's logit and probability
 };
+struct TeacherIn {           // an entry as it stands in memory
+  uint32_t x;
+  int64_t id;
+};
+__device__ __forceinline__ TeacherIn load_teacher(const Distill& h, long t, int j) {
+  if (j >= h.K) return {0u, -1};
+  const long at = t * h.K + j;
+  return {h.dtype == PV_DTYPE_F32 ? ((const uint32_t*)h.t_logits)[at] : ((const uint16_t*)h.t_logits)[at], h.ids[at]};
+}
+__device__ __forceinline__ float teacher_value(const Distill& h, uint32_t x) {
+  if (h.dtype == PV_DTYPE_F32) return as_float(x);
+  return h.dtype == PV_DTYPE_BF16 ? bf2f((uint16_t)x) : F16::up((uint16_t)x);
+}
+
+// The smallest x ^ y over the lanes that lie FROM to TO places further round in each row of 16: 0 where two ids are equal.
+template <int FROM, int TO>
+__device__ __forceinline__ uint32_t meet(int x, int y) {
+  uint32_t t = x ^ __builtin_amdgcn_update_dpp(0, y, 0x120 + FROM, 0xf, 0xf, true);      // row_ror
+  if constexpr (FROM < TO) t = min(t, meet<FROM + 1, TO>(x, y));
+  return t;
+}
+// Whether two of the first K <= 64 lanes hold the same id >= 0: all pairs, each in one direction or the other of the 8 nearest
+// places of a row of 16 lanes, rows against each other the same way.  Lists without a word twice are the rule, and a sum over
+// the list for every entry of it took 18 of 132 us at V = 1009, bf16, K = 64, 60000 rows.
+__device__ __forceinline__ bool duplicates(int id, int lane, int K) {
+  const int x = id >= 0 ? id : -1 - lane;
+  uint32_t t = meet<1, 8>(x, x);
+#pragma unroll
+  for (int o = 16; o < 64; o += 16) {
+    if (K <= (o < 32 ? 16 : 32)) break;
+    const int y = __shfl_xor(x, o);
+    t = min(t, min((uint32_t)(x ^ y), meet<1, 8>(x, y)));
+  }
+  return __ballot(t == 0) != 0;
+}
+
+// The same for longer lists, in shared memory: every entry writes its place into a table at its id's hash; one that finds
+// another's place there either holds the same id or tries again with another hash.  Every round ends with fewer entries.
+// (V = 5003, bf16, K = 200, 20000 rows: 155 us, with the sum for every entry 366.)
+__device__ __forceinline__ bool duplicates(TeacherList& l, int lane, int K) {
+  uint8_t* table = (uint8_t*)l.psum;               // 1024 places; kTeacherMax entries fit a byte
+  uint32_t factor = 0x9e3779b1u;
+  int todo = 0;                                    // entries lane, lane + 64, ...: a bit each
+  for (int j = lane; j < K; j += 64) todo |= l.id[j] >= 0 ? 1 << (j >> 6) : 0;
+  bool found = false;
+  while (__ballot(todo != 0) && !__ballot(found)) {
+    for (int j = lane; j < K; j += 64)
+      if (todo >> (j >> 6) & 1) table[(uint32_t)l.id[j] * factor >> 22] = (uint8_t)j;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int j = lane; j < K; j += 64)
+      if (todo >> (j >> 6) & 1) {
+        const int w = table[(uint32_t)l.id[j] * factor >> 22];
+        if (w != j && l.id[w] == l.id[j]) found = true;
+        if (w == j) todo &= ~(1 << (j >> 6));
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    factor += 0x3c6ef372u;                         // stays odd
+  }
+  return __ballot(found) != 0;
+}
+
+// in: entry `lane`
 template <class E>
 __device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, long t, const typename E::type* row, int lane,
-                                               TeacherList& l) {
+                                               TeacherIn in, TeacherList& l) {
   float mx = -__builtin_inff(), nan = 0.f;         // fmaxf drops a NaN: the sum keeps it
   for (int j = lane; j < h.K; j += 64) {
-    const float x = load_teacher(h, t * h.K + j);
-    const int64_t w = h.ids[t * h.K + j];
-    l.id[j] = w >= 0 && w < a.V ? (int)w : -1;
+    if (j >= 64) in = load_teacher(h, t, j);
+    const int id = in.id >= 0 && in.id < a.V ? (int)in.id : -1;
+    const float x = teacher_value(h, in.x);
+    l.z[j] = id >= 0 ? E::up(row[id]) : 0.f;
+    l.id[j] = id;
     l.p[j] = x;
     mx = fmaxf(mx, x);
     nan += x != x ? x : 0.f;
@@ -311,7 +372,7 @@ __device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, 
       if (l.id[j] < 0)
         bad = 1.f;
       else
-        zr = fmaxf(zr, E::up(row[l.id[j]]));
+        zr = fmaxf(zr, l.z[j]);
     }
   }
   sum = wave_sum(sum);
@@ -319,19 +380,25 @@ __device__ __forceinline__ Teacher teacher_row(const Rows& a, const Distill& h, 
   r.zref = finite_max(wave_max(zr));
   const float inv = r.empty ? 0.f : 1.f / sum;
   float acc = 0.f;
+  int id = -1;
   for (int j = lane; j < h.K; j += 64) {
     const float x = l.p[j], p = x == -__builtin_inff() ? 0.f : exp2_((x - mx) * h.k) * inv;
-    if (p > 0.f && l.id[j] >= 0) acc += p * (minus_log((x - mx) * h.c, sum) - a.c * (E::up(row[l.id[j]]) - r.zref));
+    id = p == 0.f ? -1 : l.id[j];
+    if (p > 0.f && id >= 0) acc += p * (minus_log((x - mx) * h.c, sum) - a.c * (l.z[j] - r.zref));
+    l.id[j] = id;
     l.p[j] = p;
   }
   r.acc = wave_sum(acc);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the lanes read each other's entries
+  const bool twice = h.K > 64 ? duplicates(l, lane, h.K) : duplicates(id, lane, h.K);
   for (int j = lane; j < h.K; j += 64) {
-    const int id = l.id[j];
-    float ps = 0.f;
-    for (int q = 0; q < h.K; ++q) ps += l.id[q] == id ? l.p[q] : 0.f;
+    float ps = l.p[j];
+    if (twice) {
+      ps = 0.f;
+      for (int q = 0; q < h.K; ++q) ps += l.id[q] == l.id[j] ? l.p[q] : 0.f;
+    }
     l.psum[j] = ps;
-    h.psum[t * h.K + j] = ps;
+    h.psum[t * h.K + j] = l.id[j] >= 0 ? ps : -1.f;
   }
   return r;
 }
@@ -475,12 +542,14 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void rows_fwd_kernel(Rows a, P
   }
   const RowIn in = load_row_in<HEAD>(a, hp, sc, t);
   const typename E::type* row = row_of<E>(a, t);
+  TeacherIn ti = {0u, -1};
+  if (HEAD == HEAD_DISTILL && tid < 64) ti = load_teacher(hd, t, tid);
   const bool bad = HEAD != HEAD_DISTILL && (y < 0 || y >= a.V);
   const float zy = HEAD != HEAD_DISTILL && !bad ? E::up(row[y]) : 0.f;
   Teacher te = {0.f, 0.f, false, false};
   __shared__ TeacherList list[HEAD == HEAD_DISTILL ? P::R : 1];
   __shared__ Stat part[1][P::W];
-  if (HEAD == HEAD_DISTILL && tid < 64) te = teacher_row<E>(a, hd, t, row, tid, list[P::slot()]);
+  if (HEAD == HEAD_DISTILL && tid < 64) te = teacher_row<E>(a, hd, t, row, tid, ti, list[P::slot()]);
   Stat st = {-__builtin_inff(), 0.f, 0.f};
   const Split<E> sp(row, a.V);
   sweep_pieces<E, ENT>(st, row + sp.head, tid, NT, sp.full, a.k);
@@ -539,6 +608,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
     return;
   }
   const RowIn in = load_row_in<HEAD>(a, hp, sc, src);
+  TeacherIn ti = {0u, -1};
+  if (HEAD == HEAD_DISTILL && tid < 64) ti = load_teacher(hd, src, tid);
   const typename E::type* row = row_of<E>(a, t);
   u32x4 raw[CH];
 #pragma unroll
@@ -553,7 +624,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
   TeacherList& list = lists[HEAD == HEAD_DISTILL ? P::slot() : 0];
   Teacher te = {0.f, 0.f, false, false};
   if (HEAD == HEAD_DISTILL && tid < 64) {
-    te = teacher_row<E>(a, hd, src, row, tid, list);
+    te = teacher_row<E>(a, hd, src, row, tid, ti, list);
     if (P::W > 1 && tid == 0) {
       flags[0] = te.empty;
       flags[1] = te.bad;
@@ -593,7 +664,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void rows_once_kernel(R
     P::sync();                                     // the list's words are written again, after the sweep
     for (int j = tid; j < hd.K; j += NT) {
       const int id = list.id[j];
-      if (id >= 0) out[id] = O::down(slope<false>(E::up(row[id]), w, a.k) + w.w * list.psum[j]);
+      if (id >= 0) out[id] = O::down(slope<false>(list.z[j], w, a.k) + w.w * list.psum[j]);
     }
   }
 }
@@ -670,10 +741,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, 8) void rows_grad_kernel(Rows 
       P::sync();                                   // the list's words are written again, after the sweep
       for (int j = tid; j < hd.K; j += NT) {
         const int64_t id = hd.ids[(long)t * hd.K + j];
-        if (id < 0 || id >= a.V) continue;
+        const float p = hd.psum[(long)t * hd.K + j];
+        if (p < 0.f || id < 0 || id >= a.V) continue;
         const int piece = (int)id - sp.head;       // of this share: its pieces, and the edges with the first
         const bool mine = piece < 0 || piece >= sp.full * E::N ? share == 0 : piece >= c0 * E::N && piece < c1 * E::N;
-        if (mine) out[id] = E::down(slope<false>(E::up(row[id]), w, a.k) + dy * hd.psum[(long)t * hd.K + j]);
+        if (mine) out[id] = E::down(slope<false>(E::up(row[id]), w, a.k) + dy * p);
       }
       P::sync();
     }

@@ -294,6 +294,29 @@ def test_distill_lists(dev):
     assert bool(torch.isnan(ops.distill_topk(z[:1], ids[:1], t[:1])))
 
 
+@pytest.mark.parametrize("K", [2, 16, 17, 33, 64, 65, 130, 256])
+def test_distill_words_listed_twice(dev, K):
+    """A word at two places of a list, a pair of places a row (all pairs up to 64 entries), and one row without such a word."""
+    from pevae_amd import ops
+    V = 300
+    i, j = torch.triu_indices(K, K, 1, device=dev)
+    if K > 64:
+        pick = torch.randperm(i.numel(), generator=torch.Generator(device=dev).manual_seed(28), device=dev)[:2000]
+        i, j = i[pick], j[pick]
+    T = i.numel() + 1
+    ids = torch.rand(T, V, generator=torch.Generator(device=dev).manual_seed(29), device=dev).topk(K, -1).indices
+    rows = torch.arange(T - 1, device=dev)
+    ids[rows, i] = ids[rows, j]
+    z = make((T, V), torch.float32, dev, 26).requires_grad_()
+    t = make((T, K), torch.float32, dev, 27)
+    loss = ops.distill_topk(z, ids, t, avg_type=None)
+    want, mag, dwant, dmag = distill64(z, ids, t, torch.ones(T, dtype=torch.bool, device=dev), 1.0, 1.0)
+    close(loss, want, mag, "loss")
+    for up in (None, torch.tensor(3.0, device=dev)):
+        k = 1.0 if up is None else 3.0
+        close(torch.autograd.grad(loss, z, up, retain_graph=True)[0], k * dwant, k * dmag, "dlogits")
+
+
 # ------------------------------------------------------------------------------------------------------------
 # policy
 # ------------------------------------------------------------------------------------------------------------
