@@ -603,17 +603,18 @@ int pv_preference_fwd(const float* logp_c, const float* ref_c, const int64_t* la
                       float smoothing, float weight, float* loss, float* rewards, float* slope, void* ws, void* stream);
 int pv_preference_bwd(const int64_t* labels_c, int Lc, const int64_t* labels_r, int Lr, long pairs, int64_t ignore,
                       const float* slope, float weight, const float* g, float* dlogp_c, float* dlogp_r, void* stream);
-/* The same loss from the logits of both answers' rows.  save_c / save_r: 4 floats a row for the backward calls, one for each
- * answer (weight for the chosen one, -weight for the rejected one; NULL: no gradient wanted).
+/* The same loss from the logits of both answers' rows.  save_c / save_r: 4 floats a row for the backward call (NULL: no gradient
+ * wanted), which leaves out an answer whose dlogits is NULL.  Answers of one type and vocabulary share their launches.
  * ws: pv_vocab_rows_ws_bytes(pairs) + 4 * pairs * (Lc + Lr) bytes. */
 int pv_preference_rows_fwd(const void* logits_c, int dtype_c, long pairs, int Lc, long s0c, long s1c, int Vc,
                            const int64_t* labels_c, const float* ref_c, const void* logits_r, int dtype_r, int Lr, long s0r,
                            long s1r, int Vr, const int64_t* labels_r, const float* ref_r, int64_t ignore, float inv_temp,
                            float beta, float smoothing, float weight, float* loss, float* rewards, float* slope, float* save_c,
                            float* save_r, void* ws, void* stream);
-int pv_preference_rows_bwd(const void* logits, int dtype, long pairs, int L, long s0, long s1, int V, const int64_t* labels,
-                           int64_t ignore, float inv_temp, const float* save, const float* slope, float weight, const float* g,
-                           void* dlogits, void* stream);
+int pv_preference_rows_bwd(const void* logits_c, int dtype_c, long pairs, int Lc, long s0c, long s1c, int Vc,
+                           const int64_t* labels_c, const void* logits_r, int dtype_r, int Lr, long s0r, long s1r, int Vr,
+                           const int64_t* labels_r, int64_t ignore, float inv_temp, const float* save_c, const float* save_r,
+                           const float* slope, float weight, const float* g, void* dlogits_c, void* dlogits_r, void* stream);
 
 /* ---- clip + skip guards + Adam over one flat buffer (main_pretrain.py:207-225,268-269;
  * dialog_models.py:122-131) ------------------------------------------------------------------------------------ */

@@ -166,7 +166,8 @@ SIGNATURES = {
     "pv_preference_bwd": (i32, [vp, i32, vp, i32, lng, i64, vp, f32, vp, vp, vp, vp]),
     "pv_preference_rows_fwd": (i32, [vp, i32, lng, i32, lng, lng, i32, vp, vp, vp, i32, i32, lng, lng, i32, vp, vp, i64, f32, f32,
                                      f32, f32, vp, vp, vp, vp, vp, vp, vp]),
-    "pv_preference_rows_bwd": (i32, [vp, i32, lng, i32, lng, lng, i32, vp, i64, f32, vp, vp, f32, vp, vp, vp]),
+    "pv_preference_rows_bwd": (i32, [vp, i32, lng, i32, lng, lng, i32, vp, vp, i32, i32, lng, lng, i32, vp, i64, f32, vp, vp, vp, f32, vp,
+                                     vp, vp, vp]),
     "pv_optim_state_bytes": (sz, []),
     "pv_grad_guard": (i32, [vp, lng, vp, f32, f32, i32, f32, f32, i32, f32, vp]),
     "pv_adam_step": (i32, [vp, vp, vp, vp, lng, vp, f32, f32, f32, f32, vp]),

@@ -3250,17 +3250,12 @@ class VocabPreferenceLoss(torch.autograd.Function):
     def backward(ctx, g, _drc, _drr):
         xc, xr, labels_c, labels_r, buf = ctx.saved_tensors
         ignore, inv_temp, weight, at = ctx.meta
-        save = _p(buf)
-        slope = save + at
-        out = []
-        for x, labels, w in ((xc, labels_c, weight), (xr, labels_r, -weight)):
-            d = None
-            if x is not None:
-                d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                _launch(x.device, "pv_preference_rows_bwd", *_row_args(x), _p(labels), ignore, inv_temp, save, slope, w, _p(g), _p(d))
-            out.append(d)
-            save += 16 * labels.numel()            # (the chosen answer's rows lie before the rejected one's)
-        return tuple(out) + (None,) * 11
+        save, absent = _p(buf), (None, 0, labels_c.shape[0], 1, 0, 0, 1)
+        ac, ar = (absent if x is None else _row_args(x) for x in (xc, xr))
+        dc, dr = (None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (xc, xr))
+        _launch(buf.device, "pv_preference_rows_bwd", *ac, _p(labels_c), *ar[:2], *ar[3:], _p(labels_r), ignore, inv_temp, save,
+                save + 16 * labels_c.numel(), save + at, weight, _p(g), _p(dc), _p(dr))
+        return (dc, dr) + (None,) * 11
 
 
 def _preference_args(shape_c, shape_r, chosen_labels, rejected_labels, ref_chosen, ref_rejected, label_smoothing, avg_type):

@@ -549,6 +549,29 @@ def test_vocab_preference_loss(dev, dtype, P, Lc, Lr, V, smooth, with_ref, avg):
     assert torch.equal(only, torch.autograd.grad(loss, zr)[0])
 
 
+@pytest.mark.parametrize("V", [200, 5003])
+def test_vocab_preference_one_answer_or_two_kinds(dev, V):
+    """A gradient for one answer only, and answers of different types and vocabularies, are what two launches of their own give:
+    the token log-probabilities and their loss do the same arithmetic."""
+    from pevae_amd import ops
+    P, Lc, Lr = 4, 5, 3
+    yc, yr = labels_of((P, Lc), V, dev, 170), labels_of((P, Lr), V, dev, 171)
+    for kinds in ((torch.bfloat16, V, torch.bfloat16, V), (torch.bfloat16, V, torch.float32, V), (torch.float16, V, torch.float16, V + 9)):
+        zc, zr = make((P, Lc, kinds[1]), kinds[0], dev, 172), make((P, Lr, kinds[3]), kinds[2], dev, 173)
+        got = {}
+        for need_c, need_r in ((True, True), (True, False), (False, True)):
+            xc, xr = zc.clone().requires_grad_(need_c), zr.clone().requires_grad_(need_r)
+            loss = ops.vocab_preference_loss(xc, yc, xr, yr, ignore_index=-7)[0]
+            loss.backward()
+            got[need_c, need_r] = loss.detach(), xc.grad, xr.grad
+        xc, xr = zc.clone().requires_grad_(), zr.clone().requires_grad_()
+        loss = ops.preference_loss(ops.token_logprobs(xc, yc, -7), yc, ops.token_logprobs(xr, yr, -7), yr, ignore_index=-7)[0]
+        loss.backward()
+        for (need_c, need_r), (l, dc, dr) in got.items():
+            assert torch.equal(l, loss.detach())
+            assert (torch.equal(dc, xc.grad) if need_c else dc is None) and (torch.equal(dr, xr.grad) if need_r else dr is None)
+
+
 def test_preference_far_apart(dev):
     """Rewards far apart: the loss is 0 or the distance, without overflow; infinite ones stay infinite."""
     from pevae_amd import ops

@@ -137,6 +137,12 @@ def test_entry_points_refuse_on_the_host():
     assert lib.pv_colsum_scaled_bf16(p, 7, 4, 7, p, p, p, None) == -1 and lib.pv_scale_by_f32(p, 6, p, None) == -1
     assert lib.pv_preference_rows_fwd(p, 0, 2, 3, 15, 5, 5, p, None, p, 0, 0, 15, 5, 5, p, None, 0, 1.0, 0.1, 0.0, 1.0, p, p, p, p, p, p,
                                       None) == -1
-    assert lib.pv_preference_rows_bwd(p, 0, 2, 3, 15, 5, 5, p, 0, 1.0, None, p, 1.0, p, p, None) == -1
+
+    def preference_bwd(save_c=p, save_r=p, dc=p, dr=p, Vr=5, dtype_r=0):
+        return lib.pv_preference_rows_bwd(p, 0, 2, 3, 15, 5, 5, p, p, dtype_r, 3, 15, 5, Vr, p, 0, 1.0, save_c, save_r, p, 1.0, p, dc, dr,
+                                          None)
+
+    for bad in (dict(save_c=None), dict(save_r=None), dict(dc=None, dr=None), dict(Vr=0), dict(dtype_r=4)):
+        assert preference_bwd(**bad) == -1, bad
     assert lib.pv_distill_max_entries() == 256 == ops.DISTILL_MAX
     assert lib.pv_vocab_rows_ws_bytes(10) >= 160
