@@ -1016,3 +1016,59 @@ def test_decoder_learns_from_a_teacher_and_from_judgments(dev):
     for a, b in zip(*roads):
         for i in (1, 2):
             assert float((a[i] - b[i]).abs().max()) <= 2e-2 * float(b[i].abs().max())
+
+
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("drop", [0.0, 0.3])
+def test_losses_of_one_forward_pass_add_up(dev, sink, drop):
+    """The NLL, distillation, a policy loss and one with an entropy bonus on ONE decoder output, backward in one pass with the
+    framework's side streams, with and without gradients that are accumulated into: the sum of the gradients of each alone,
+    under the same dropout masks (a mask goes by the generator's step and the call's number: nothing advances the one, and the
+    other starts at 0 for every pass).  The projection's gradients are sums of the same fp32 terms (V, H and B L of them: 1e-4 of
+    the largest is granted); what passes the recurrence is rounded to bf16 on the way, once for the sum and once for each
+    alone.  A policy loss in front of the NLL shares its node, whose weight gradient rounds p_v g_t to bf16: once for the sum of
+    both g, once for each alone, half a step (2^-8) of |p_v g_t| at most each, so that an element is off by no more than
+    2 * 2^-8 * sum_t |p_v - [v = y_t]| |g_t| |h_t|, with |h| <= 1 / (1 - drop)."""
+    from pevae_amd import criterions, ops
+    from pevae_amd.dls_vae import DLSVAE
+    from pevae_amd.enc2dec import decoders as D
+    torch.manual_seed(11)
+    V, L, E, H, B = 5003, 12, 64, 512, 8
+    dec = D.DecoderRNN(V, L, E, H, 1, 2, 3, rnn_cell="gru", dropout_p=drop, input_dropout_p=drop,
+                       embedding=torch.nn.Embedding(V, E, padding_idx=0)).to(dev).train()
+    ids = torch.randint(4, V, (B, L), device=dev)
+    y = torch.cat([ids[:, 1:], torch.zeros(B, 1, dtype=torch.long, device=dev)], 1)
+    y[1, 5:], y[6, 1:] = 0, 0
+    h0 = (torch.randn(1, B, H, device=dev) * 0.3).requires_grad_()
+    teacher = torch.randn(B, L, V, device=dev).topk(8, -1)
+    adv = torch.randn(B, device=dev)
+    with torch.no_grad():
+        old = criterions.token_log_probs(dec(B, ids, h0, mode=D.TEACH_FORCE)[0], y, 0) - 0.1
+    losses = [lambda o: criterions.NLLEntropy(0, None)(o, y),
+              lambda o: criterions.TopKDistill(0, None, weight=0.5)(o, y, teacher.indices, teacher.values),
+              lambda o: criterions.ClippedPolicyLoss(0, None)(o, y, old, adv)[0],
+              lambda o: criterions.ClippedPolicyLoss(0, None, ent_coef=0.1)(o, y, old, adv)[0]]
+    params = [p for p in dec.parameters()] + [h0]
+
+    def grads(chosen):
+        for p in params:
+            p.grad = torch.zeros_like(p) if sink else None
+        for m in dec.modules():
+            if isinstance(m, ops.Dropout):
+                m.calls = 0
+        out = dec(B, ids, h0, mode=D.TEACH_FORCE)[0]
+        terms = [f(out) for f in chosen]
+        DLSVAE._run_backward(lambda: torch.autograd.backward(terms))
+        return [p.grad.clone() for p in params]
+
+    alone = [grads([f]) for f in losses]
+    lp = (old + 0.1).requires_grad_()
+    g = 1.0 / B + float(torch.autograd.grad(ops.policy_loss(lp, y, old, adv, ignore_index=0)[0], lp)[0].abs().max()) * 4
+    count = torch.bincount(y[y != 0], minlength=V).max()         # rows that have a word as their target; p adds less than 1 to them
+    shared = 2 * 2.0 ** -8 * (float(count) + 1) * g / (1 - drop)
+    for chosen in ((0, 1, 2, 3), (3, 2, 1, 0), (0, 1)):
+        for p, got, *each in zip(params, grads([losses[k] for k in chosen]), *[alone[k] for k in chosen]):
+            want, top = sum(each), max(float(e.abs().max()) for e in each)
+            share = 1e-4 if p is dec.project.weight or p is dec.project.bias else 2e-2
+            extra = shared if chosen == (3, 2, 1, 0) and p is dec.project.weight else 0.0
+            assert float((got - want).abs().max()) <= share * len(each) * top + extra
