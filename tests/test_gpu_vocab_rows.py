@@ -894,6 +894,22 @@ def test_dead_rows_behind_a_projection_hold_anything(dev, shape):
         assert bool(torch.isfinite(a).all()) and torch.equal(a, c)
 
 
+def test_more_projected_logits_than_32_bits_count(dev):
+    """The last rows of 27000 x 81900 logits (2.2e9, behind the 2^31st) have the gradient that they have alone, rows and products
+    being the same; sums in another order move it by 1e-5 of the largest at most."""
+    from pevae_amd import ops
+    T, V, H, K = 27000, 81900, 64, 4
+    hid, w, b = (make(s, torch.float32, dev, k, 0.3) for k, s in ((240, (1, T, H)), (241, (V, H)), (242, (V,))))
+    ids = torch.randint(0, V // 2, (1, T, 1), generator=torch.Generator(device=dev).manual_seed(243), device=dev) + torch.arange(K, device=dev)
+    t = make((1, T, K), torch.float32, dev, 244)
+    grads = []
+    for at in (0, T - 8):
+        x = hid[:, at:].clone().requires_grad_()
+        loss = ops.projected_distill_topk(x, w, b, ids[:, at:].contiguous(), t[:, at:].contiguous(), avg_type=None)
+        grads.append(torch.autograd.grad(loss, x)[0][0, -8:])
+    assert float((grads[0] - grads[1]).abs().max()) <= 1e-5 * float(grads[1].abs().max())
+
+
 def test_labels_of_deferred_rows(dev):
     """Labels of any integer type and stride (views of one storage among them), and their refusals."""
     from pevae_amd.enc2dec import decoders as D
