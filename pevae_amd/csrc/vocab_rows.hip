@@ -256,7 +256,7 @@ struct PolicyTerm {
 __device__ __forceinline__ PolicyTerm policy_term(const Policy& h, float lp, float old_lp, float ref_lp, float A) {
   const float r = expf(lp - old_lp);
   float u = r * A, w = fminf(fmaxf(r, h.lo), h.hi) * A;
-  if (A == 0.f) u = w = 0.f;                      // r may be infinite
+  if (A == 0.f && r == r) u = w = 0.f;            // r may be infinite; a NaN stays
   PolicyTerm o;
   const bool cut = u > w;
   o.cut = cut ? 1.f : 0.f;
