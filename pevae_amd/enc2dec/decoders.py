@@ -77,16 +77,34 @@ class DeferredLogProbs(object):
         self._nll_cache = {}
         self._nll_labels = []
 
+    def _kept(self, key, make, keep=lambda res: True):
+        """The result of make() for `key`, made once.  One made without gradients (under torch.no_grad(): the scores of an old
+        policy, an evaluation) has no history and serves only callers that ask for none; one with a history serves all."""
+        on = torch.is_grad_enabled()
+        for mode in (True,) if on else (True, False):
+            hit = self._nll_cache.get((mode, key))
+            if hit is not None:
+                return hit
+        res = make()
+        if keep(res):
+            self._nll_cache[on, key] = res
+        return res
+
+    @staticmethod
+    def _key(name, labels, ignore_index):
+        return name, labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index
+
     # -- what the criterions use -------------------------------------------------------------------------
     def token_nll(self, labels, ignore_index, sums_only=False):
         """(nll_tok, targets in row order): per-token -log p[label] (0 where label == ignore_index) without the logits.
         sums_only: the caller only wants {sum, live count}; where the fused kernels run, the first result is then that pair
         already (third result True) and the per-token vector is never put back into the caller's row order."""
-        key = (labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
-        hit = self._nll_cache.get(key)
-        if hit is not None:
-            return hit + (False,)
-        self._nll_labels.append(labels)          # the cache goes by address: no other labels may come to lie there
+        # a sum alone is not kept as the tokens' values
+        return self._kept(self._key("nll", labels, ignore_index), lambda: self._token_nll(labels, ignore_index, sums_only),
+                          lambda res: not res[2])
+
+    def _token_nll(self, labels, ignore_index, sums_only):
+        self._nll_labels.append(labels)          # results go by the labels' address: no other labels may come to lie there
         B, L, H = self.hid.shape
         if self.hid_bf16 is not None or (self.drop is not None and self.layout is not None):
             Lh, Bh, Bpad = self.layout
@@ -109,19 +127,14 @@ class DeferredLogProbs(object):
             tgt = labels.reshape(-1)
             nll, _ = ops.VocabNLL.apply(self.hid.reshape(B * L, H), self.weight, self.bias, tgt, self.inv_temp,
                                         ignore_index, None, None, None, None, sums_only)
-        if sums_only and ops.VocabNLL.RETURNED_SUMS:     # the op says which form it returned (T = 2 rows look the same)
-            return nll, tgt, True
-        res = (nll, tgt)
-        self._nll_cache[key] = res
-        return res + (False,)
+        # the op says which form it returned (T = 2 rows look the same)
+        return nll, tgt, sums_only and ops.VocabNLL.RETURNED_SUMS
 
     def _sums(self, labels, ignore_index):
-        key = ("sums", labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
-        hit = self._nll_cache.get(key)
-        if hit is None:
+        def make():
             out, tgt, is_sums = self.token_nll(labels, ignore_index, sums_only=SUMS_ONLY)
-            hit = self._nll_cache[key] = out if is_sums else ops.MaskedSum.apply(out, tgt, ignore_index)
-        return hit
+            return out if is_sums else ops.MaskedSum.apply(out, tgt, ignore_index)
+        return self._kept(self._key("sums", labels, ignore_index), make)
 
     def token_nll_sums(self, labels, ignore_index):
         """(sum of the token NLL, number of non-ignored tokens) as device scalars; NLLEntropy and Perplexity of one step
@@ -132,11 +145,8 @@ class DeferredLogProbs(object):
     def loss_head(self, labels, ignore_index):
         """(NLLEntropy avg_type 'seq', Perplexity) of these labels as device scalars, one launch for both (ops.NllHead);
         the two criterions of a step ask for one each."""
-        key = ("head", labels.data_ptr(), labels._version, tuple(labels.shape), labels.stride(), ignore_index)
-        hit = self._nll_cache.get(key)
-        if hit is None:
-            hit = self._nll_cache[key] = ops.NllHead.apply(self._sums(labels, ignore_index), self.hid.shape[0])
-        return hit
+        return self._kept(self._key("head", labels, ignore_index),
+                          lambda: ops.NllHead.apply(self._sums(labels, ignore_index), self.hid.shape[0]))
 
     def token_logp(self, labels, ignore_index):
         """Log-probability of `labels` [B, L] (0 where label == ignore_index) without the logits, differentiable."""
@@ -154,12 +164,14 @@ class DeferredLogProbs(object):
 
     # -- dense fallback: behaves like the reference's tensor ---------------------------------------------------
     def materialize(self):
-        if self._dense is None:
-            B, L, H = self.hid.shape
-            hid = self.projection()[0]
-            flat = ops.VocabLogProbDense.apply(hid.reshape(B * L, H), self.weight, self.bias, self.inv_temp)
-            self._dense = flat.view(B, L, -1)
+        self._dense = self._kept("dense", self._make_dense)
         return self._dense
+
+    def _make_dense(self):
+        B, L, H = self.hid.shape
+        hid = self.projection()[0]
+        flat = ops.VocabLogProbDense.apply(hid.reshape(B * L, H), self.weight, self.bias, self.inv_temp)
+        return flat.view(B, L, -1)
 
     def size(self, dim=None):
         shape = torch.Size((self.hid.shape[0], self.hid.shape[1], self.weight.shape[0]))
