@@ -545,7 +545,7 @@ def precompact_targets(labels, layout, ignore_index):
         tgt = labels.reshape(-1).contiguous()
     T = tgt.numel()
     perm = count = None
-    if SKIP_IGNORED_TOKENS and ignore_index >= 0:
+    if _skips_ignored(ignore_index):
         perm = torch.empty(T, dtype=torch.int64, device=tgt.device)
         count = torch.empty(1, dtype=torch.int32, device=tgt.device)
         _lib.call("pv_vocab_compact", _p(tgt), T, ignore_index, _p(perm), _p(count), _stream())
@@ -814,6 +814,14 @@ def _vocab_operands(hid, weight):
 
 
 SKIP_IGNORED_TOKENS = os.environ.get("PEVAE_VOCAB_DENSE", "0") != "1"     # see VocabNLL
+
+
+def _skips_ignored(ignore_index):
+    """Whether VocabNLL moves the ignored rows out of the way.  A negative index usually marks nothing (-1, -100); one beyond the
+    fused kernels' 32-bit labels (pv_vocab_gather32 brings all such labels to -2147483647) is told apart here only."""
+    return SKIP_IGNORED_TOKENS and (ignore_index >= 0 or ignore_index <= -2147483647)
+
+
 # H = 512 with gradients wanted: the two flash-attention-shaped kernels of csrc/vocab_fused.hip (no [T, V] matrix in HBM in
 # either pass) instead of the four tile GEMMs with the P / P^T round trip.  PEVAE_VOCAB_FUSED=0 keeps the tile-GEMM path.
 FUSED_VOCAB = os.environ.get("PEVAE_VOCAB_FUSED", "1") != "0"
@@ -869,7 +877,7 @@ class VocabNLL(torch.autograd.Function):
         if FUSED_VOCAB and any(ctx.needs_input_grad[:3]) and _lib.load().pv_vocab_fused_supported(Hp):
             return VocabNLL._forward_fused(ctx, hid, weight, bias, target, inv_temp, ignore_index, T, H, V, Hp, h_bf, ldh, w_bf,
                                            pre, sums_only)
-        if SKIP_IGNORED_TOKENS and ignore_index >= 0:
+        if _skips_ignored(ignore_index):
             if pre is not None and pre[0] is not None:
                 perm, count = pre
             else:
@@ -910,7 +918,7 @@ class VocabNLL(torch.autograd.Function):
         dev = weight.device
         perm = count = t_c = None
         t32 = torch.empty(T, dtype=torch.int32, device=dev)
-        if SKIP_IGNORED_TOKENS and ignore_index >= 0:
+        if _skips_ignored(ignore_index):
             if pre is not None and pre[0] is not None:      # (perm, count) made ahead by precompact_targets()
                 perm, count = pre
             else:

@@ -78,3 +78,19 @@ def test_scoring_and_training_on_one_output(dev, H, V, route):
         for p, w in zip(params, want):
             assert (p.grad is None) == (w is None) and (w is None or torch.equal(p.grad, w))
         assert float(dec.project.weight.grad.abs().max()) > 0
+
+
+def test_ignored_labels_of_any_number(dev):
+    """Rows of an ignored label are dead whatever its number, also where it does not fit 32 bits."""
+    from pevae_amd.enc2dec import decoders as D
+    gen = torch.Generator(device=dev).manual_seed(31)
+    for H, V in PATHS:
+        hid, w, b = (torch.randn(*s, generator=gen, device=dev) * 0.3 for s in ((2, 5, H), (V, H), (V,)))
+        w.requires_grad_()
+        y = torch.randint(1, V, (2, 5), generator=gen, device=dev)
+        want = D.DeferredLogProbs(hid, w, b, 1.0).token_logp(y, 0)
+        for ignore in (-1, V, V + 9, -100, 1 << 40, -(1 << 40)):
+            dead = y.clone()
+            dead[1, 2:] = ignore
+            got = D.DeferredLogProbs(hid, w, b, 1.0).token_logp(dead, ignore)
+            assert float(got[1, 2:].abs().max()) == 0.0 and torch.equal(got[0], want[0]) and torch.equal(got[1, :2], want[1, :2]), ignore
