@@ -67,8 +67,8 @@ int pv_gemm_bf16_tn_splitk(const void* A, int lda, const void* B, int ldb, int M
 
 /* ---- fused vocabulary projection + log-softmax + NLL -----------------------------------------------------
  * Forward: logits = (h W^T + bias) * inv_temp are produced tile-wise by the MFMA GEMM and reduced on the fly
- * to per-token lse[t] and nll[t] = lse - logit[target] (0 where target == ignore_index); the [T,V] log-prob
- * tensor is never written.  Replaces decoders.py:191-193 (Linear + /temperature + log_softmax) fused with
+ * to per-token lse[t] and nll[t] = lse - logit[target] (0 where target == ignore_index, NaN where any other is
+ * outside [0, V)); the [T,V] log-prob tensor is never written.  Replaces decoders.py:191-193 (Linear + /temperature + log_softmax) fused with
  * criterions.py:55-64 (NLLLoss sum) and criterions.py:133-138 (Perplexity's token mean).
  * h [T][ldh] bf16, W [V][ldw] bf16, H % 64 == 0. */
 size_t pv_vocab_nll_fwd_ws_bytes(int T, int V);
@@ -96,12 +96,12 @@ int pv_scatter_rows_f32(const float* src, long lds, const int64_t* perm, const i
 /* ---- the same group with NOTHING of size [T][V] in HBM, forward and backward (H = 512; pv_vocab_fused_supported) ------
  * Two flash-attention-shaped kernels (csrc/vocab_fused.hip), each two chained MFMA products per 32 x 32 block with the
  * probabilities handed from the first product's accumulator to the second's operand in registers:
- *   pv_vocab_fused_fwd : S^T = W h^T -> online softmax -> O^T += W^T P^T.  Emits lse[t], nll[t] (0 for ignored rows) AND
+ *   pv_vocab_fused_fwd : S^T = W h^T -> online softmax -> O^T += W^T P^T.  Emits lse[t], nll[t] (as above) AND
  *                        U[t][:] = sum_v softmax[t,v] W[v] - W[target[t]] (fp32 [T][512]), the gradient of nll[t] with
  *                        respect to the SCALED logits' input h[t] / inv_temp: dH[t] = dL/dnll[t] * inv_temp * U[t], an
  *                        elementwise pass in backward (pv_scatter_rows_scaled_f32) instead of a GEMM over a stored P.
  *   pv_vocab_fused_dw  : S = h W^T -> P = gscale (softmax - onehot) -> Z += P^T h.  Emits dW (+= when accumulate) and dbias;
- *                        gscale[t] = dL/dnll[t] (0 for ignored rows; pv_vocab_gscale), lse from the forward call.
+ *                        gscale[t] = dL/dnll[t] (0 for ignored rows; pv_vocab_row_scale), lse from the forward call.
  * Rows are the compact order of pv_vocab_compact (live rows first; live_rows = its count, NULL = all T rows);
  * target32: the targets as int32 (pv_vocab_gather32).  Replaces decoders.py:191-193 + criterions.py:55-64 and their
  * backward.  workspace: pv_vocab_fused_{fwd,dw}_ws_bytes -- per-workgroup partial results of the stream-K split, folded
@@ -322,6 +322,10 @@ int pv_nll_head_bwd(const float* sums2, const float* out2, const float* g_nll, c
                     void* stream);
 int pv_vocab_gscale(const float* dnll, const int64_t* perm, const int64_t* target, int64_t ignore, int T, float* gscale,
                     void* stream);
+/* The same row scale with the targets looked at: NaN where a live one is outside [0, V), whose nll[t] the forward calls make NaN
+ * too.  one != 0: dnll[0] is every live row's upstream gradient (of a sum). */
+int pv_vocab_row_scale(const float* dnll, int one, const int64_t* perm, const int64_t* target, int64_t ignore, int V, int T,
+                       float* gscale, void* stream);
 /* dense-input NLL (criterions.py:57-63 on a materialised log-prob tensor): out[t] = -logp[t][target[t]] */
 int pv_pick_nll_fwd(const float* logp, const int64_t* target, int64_t ignore, int T, int V, float* out,
                     void* stream);

@@ -110,6 +110,7 @@ SIGNATURES = {
     "pv_colsum_f32": (i32, [vp, i32, lng, i32, vp, i32, vp]),
     "pv_masked_sum_bwd": (i32, [vp, i64, vp, lng, vp, vp]),
     "pv_vocab_gscale": (i32, [vp, vp, vp, i64, i32, vp, vp]),
+    "pv_vocab_row_scale": (i32, [vp, i32, vp, vp, i64, i32, i32, vp, vp]),
     "pv_masked_sum": (i32, [vp, vp, i64, lng, vp, vp]),
     "pv_sum_group": (i32, [vp, vp]),
     "pv_nll_head_fwd": (i32, [vp, i32, vp, vp]),

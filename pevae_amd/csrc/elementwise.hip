@@ -711,11 +711,15 @@ __global__ void masked_sum_bwd_kernel(const int64_t* __restrict__ mask, int64_t 
   for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x)
     dx[i] = (!mask || mask[i] != ignore) ? gv : 0.f;
 }
-// row scale of the vocabulary backward: gscale[t] = dnll[perm ? perm[t] : t] * (target[t] != ignore)
-__global__ void vocab_gscale_kernel(const float* __restrict__ dnll, const int64_t* __restrict__ perm,
-                                    const int64_t* __restrict__ target, int64_t ignore, int T, float* __restrict__ gscale) {
-  for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < T; t += gridDim.x * blockDim.x)
-    gscale[t] = target[t] != ignore ? dnll[perm ? perm[t] : t] : 0.f;
+// row scale of the vocabulary backward: gscale[t] = dnll[perm ? perm[t] : t] * (target[t] != ignore), or the one value dnll[0]
+// for every live row; NaN where a live target is outside [0, V) (V = 0: not looked at)
+__global__ void vocab_gscale_kernel(const float* __restrict__ dnll, int one, const int64_t* __restrict__ perm,
+                                    const int64_t* __restrict__ target, int64_t ignore, int64_t V, int T,
+                                    float* __restrict__ gscale) {
+  for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < T; t += gridDim.x * blockDim.x) {
+    const int64_t y = target[t];
+    gscale[t] = y == ignore ? 0.f : V == 0 || (y >= 0 && y < V) ? dnll[one ? 0 : perm ? perm[t] : t] : __builtin_nanf("");
+  }
 }
 }  // namespace
 
@@ -732,8 +736,17 @@ int pv_masked_sum_bwd(const int64_t* mask, int64_t ignore, const float* g, long 
 int pv_vocab_gscale(const float* dnll, const int64_t* perm, const int64_t* target, int64_t ignore, int T, float* gscale,
                     void* stream) {
   PV_REQUIRE(dnll && target && gscale && T > 0, "pv_vocab_gscale: bad argument");
-  hipLaunchKernelGGL(vocab_gscale_kernel, dim3(grid_for(T, 256)), dim3(256), 0, (hipStream_t)stream, dnll, perm, target,
-                     ignore, T, gscale);
+  hipLaunchKernelGGL(vocab_gscale_kernel, dim3(grid_for(T, 256)), dim3(256), 0, (hipStream_t)stream, dnll, 0, perm, target,
+                     ignore, (int64_t)0, T, gscale);
+  PV_LAUNCH_CHECK("vocab_gscale_kernel");
+  return PV_OK;
+}
+
+int pv_vocab_row_scale(const float* dnll, int one, const int64_t* perm, const int64_t* target, int64_t ignore, int V, int T,
+                       float* gscale, void* stream) {
+  PV_REQUIRE(dnll && target && gscale && T > 0 && V > 0, "pv_vocab_row_scale: bad argument");
+  hipLaunchKernelGGL(vocab_gscale_kernel, dim3(grid_for(T, 256)), dim3(256), 0, (hipStream_t)stream, dnll, one, perm, target,
+                     ignore, (int64_t)V, T, gscale);
   PV_LAUNCH_CHECK("vocab_gscale_kernel");
   return PV_OK;
 }

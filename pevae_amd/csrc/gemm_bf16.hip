@@ -705,11 +705,12 @@ struct EpiLogProb {
   }
 };
 
+// A live row whose target is no word of the vocabulary has the NLL NaN (its target logit was never written).
 // combine the per-slab (max, sumexp) partials: 16 rows per block, 16 slab-strided lanes per row (a lane's dependent
 // chain is nslab/16 = 20 links at the Yelp vocabulary), then the 16 lane results of a row in lane order through LDS
 __global__ __launch_bounds__(256) void vocab_reduce_kernel(const float2* __restrict__ part,
                                                             const float* __restrict__ tgt_logit,
-                                                            const int64_t* __restrict__ target, int T,
+                                                            const int64_t* __restrict__ target, int T, int V,
                                                             int Tpad, int nslab, int64_t ignore_index,
                                                             const int* __restrict__ live_rows,
                                                             float* __restrict__ lse,
@@ -749,7 +750,7 @@ __global__ __launch_bounds__(256) void vocab_reduce_kernel(const float2* __restr
     const float l = M + logf(S);
     lse[row] = l;
     const int64_t t = target[row];
-    nll[row] = (t == ignore_index) ? 0.f : l - tgt_logit[row];
+    nll[row] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - tgt_logit[row] : __builtin_nanf("");
   }
 }
 
@@ -1243,13 +1244,11 @@ int pv_vocab_nll_fwd(const void* h, int ldh, const void* W, int ldw, const float
   float2* part = (float2*)workspace;
   float* tgt_logit = (float*)(part + (size_t)nslab * Tpad);
   hipStream_t st = (hipStream_t)stream;
-  // rows whose target is out of range (e.g. ignore_index < 0) never get a target logit written
-  PV_HIP(hipMemsetAsync(tgt_logit, 0, (size_t)Tpad * sizeof(float), st));
   GemmArgs g{(const bf16_t*)h, (const bf16_t*)W, T, V, H, ldh, ldw, 1, 0, live_rows, nullptr};
   EpiSoftmax e{bias, target, part, tgt_logit, T, V, Tpad, inv_temp};
   rc = big_tile(T, V, H) ? launch<decltype(e), 4>(g, e, st, "pv_vocab_nll_fwd") : launch(g, e, st, "pv_vocab_nll_fwd");
   if (rc) return rc;
-  hipLaunchKernelGGL(vocab_reduce_kernel, dim3(cdiv(T, 16)), dim3(256), 0, st, part, tgt_logit, target, T,
+  hipLaunchKernelGGL(vocab_reduce_kernel, dim3(cdiv(T, 16)), dim3(256), 0, st, part, tgt_logit, target, T, V,
                      Tpad, nslab, ignore_index, live_rows, lse, nll);
   PV_LAUNCH_CHECK("vocab_reduce_kernel");
   return PV_OK;

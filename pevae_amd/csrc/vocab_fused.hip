@@ -612,10 +612,11 @@ __global__ __launch_bounds__(256) void vocab_fwd_combine_kernel(FwdCombineArgs a
     invL[tid] = 1.f / L;
     const int t = rg * UNIT + tid;
     if (blockIdx.y == 0 && t < a.T) {
-      const bool is_live = t < nlive && (long)a.target[t] != a.ignore_index;
+      const int y = a.target[t];
+      const bool is_live = t < nlive && (long)y != a.ignore_index;
       const float lse = M + logf(L);
       a.lse[t] = t < nlive ? lse : 0.f;
-      a.nll[t] = is_live ? lse - tl : 0.f;
+      a.nll[t] = !is_live ? 0.f : y >= 0 && y < a.V ? lse - tl : __builtin_nanf("");     // a target that is no word: NaN
     }
   }
   __syncthreads();

@@ -834,6 +834,8 @@ class VocabNLL(torch.autograd.Function):
     """nll_tok[t] = -log_softmax((h W^T + b) / temperature)[target[t]], 0 for ignored targets; the [T,V]
     log-prob tensor is never built (decoders.py:191-193 + criterions.py:55-64 of the reference, fused).
 
+    A live target outside [0, V) makes its token's NLL, and with it every gradient that the row enters, NaN.
+
     Rows whose target is the ignore index add exactly zero to the loss and to every gradient (NLLLoss(ignore_index),
     criterions.py:38-41), so by default they are not multiplied at all: a stable partition moves the live rows to the
     front (pv_vocab_compact / pv_vocab_gather) and the four GEMMs of the group take the live-row count from device
@@ -972,12 +974,9 @@ class VocabNLL(torch.autograd.Function):
         T, H, V, Hp, ldh, inv_temp, ignore_index = ctx.dims
         dev = w_bf.device
         gscale = torch.empty(T, dtype=torch.float32, device=dev)      # `target` is already in compact order
-        if ctx.sums_only:            # dnll = d{sum, count}: every live row's upstream gradient is d sum
-            _lib.call("pv_masked_sum_bwd", _p(target), ignore_index, _p(dnll.to(torch.float32).contiguous()), T, _p(gscale),
-                      _stream())
-        else:
-            _lib.call("pv_vocab_gscale", _p(dnll.to(torch.float32).contiguous()), _p(perm), _p(target), ignore_index, T,
-                      _p(gscale), _stream())
+        # (sums_only: dnll = d{sum, count}, every live row's upstream gradient is d sum)
+        _lib.call("pv_vocab_row_scale", _p(dnll.to(torch.float32).contiguous()), int(ctx.sums_only), _p(perm), _p(target),
+                  ignore_index, V, T, _p(gscale), _stream())
         dH = torch.empty((T, H), dtype=torch.float32, device=dev)
         if ctx.drop is not None and FUSE_DROP_SCATTER and T % ctx.drop[3][2] == 0:
             # the output dropout's backward rides in the scatter's store pass (one pass over dH instead of two)
@@ -1042,8 +1041,8 @@ class VocabNLL(torch.autograd.Function):
         dev = w_bf.device
         Tp, Vp = round_up(T, 64), round_up(V, 64)
         gscale = torch.empty(T, dtype=torch.float32, device=dev)      # `target` is already in compact order
-        _lib.call("pv_vocab_gscale", _p(dnll.to(torch.float32).contiguous()), _p(perm), _p(target), ignore_index, T, _p(gscale),
-                  _stream())
+        _lib.call("pv_vocab_row_scale", _p(dnll.to(torch.float32).contiguous()), 0, _p(perm), _p(target), ignore_index, V, T,
+                  _p(gscale), _stream())
         P = workspace("vocab_P", Tp * Vp, BF16, dev)
         PT = workspace("vocab_PT", Vp * Tp, BF16, dev)
         dbp = workspace("vocab_dbias_part", (Tp // 64) * Vp, torch.float32, dev)

@@ -94,3 +94,73 @@ def test_ignored_labels_of_any_number(dev):
             dead[1, 2:] = ignore
             got = D.DeferredLogProbs(hid, w, b, 1.0).token_logp(dead, ignore)
             assert float(got[1, 2:].abs().max()) == 0.0 and torch.equal(got[0], want[0]) and torch.equal(got[1, :2], want[1, :2]), ignore
+
+
+BAD = (lambda V: V, lambda V: -1, lambda V: (1 << 40) + 5, lambda V: -(1 << 50))
+
+
+@pytest.mark.parametrize("H,V", PATHS + [(512, 4096 + 77)])
+@pytest.mark.parametrize("ignore", [0, -7])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_labels_that_name_no_word(dev, H, V, ignore, frozen):
+    """A live label outside [0, V) has a NaN log-probability and a NaN gradient of its state; the other rows keep theirs.  With
+    frozen states and weights the kernel without a backward pass runs."""
+    from pevae_amd import criterions, ops
+    from pevae_amd.enc2dec import decoders as D
+    gen = torch.Generator(device=dev).manual_seed(30)
+    B, L = 3, 7
+    hid, w, b = (torch.randn(*s, generator=gen, device=dev) * 0.3 for s in ((B, L, H), (V, H), (V,)))
+    xs = hid, w, b = [x.requires_grad_(not frozen) for x in (hid, w, b)]
+    y = torch.randint(1, V, (B, L), generator=gen, device=dev)
+    y[0, 5:], y[2, 2] = ignore, ignore
+    places = [(0, 1), (1, 0), (1, 6), (2, 4)]
+    bad = y.clone()
+    for (i, j), f in zip(places, BAD):
+        bad[i, j] = f(V)
+    hit = bad != y
+    want = D.DeferredLogProbs(hid, w, b, 1.0).token_logp(y, ignore)
+    out = D.DeferredLogProbs(hid, w, b, 1.0)
+    got = out.token_logp(bad, ignore)
+    assert torch.equal(torch.isnan(got), hit) and torch.equal(got[~hit], want[~hit])
+    old, adv = (want.detach() - 0.1), torch.ones(B, device=dev)
+    for loss in (criterions.NLLEntropy(ignore, None)(out, bad), criterions.ClippedPolicyLoss(ignore, None)(out, bad, old, adv)[0],
+                 criterions.NLLEntropy(ignore, None)(D.DeferredLogProbs(hid, w, b, 1.0), bad),
+                 criterions.ClippedPolicyLoss(ignore, None)(D.DeferredLogProbs(hid, w, b, 1.0), bad, old, torch.zeros(B, device=dev))[0],
+                 criterions.PreferenceLoss(ignore, None)(D.DeferredLogProbs(hid, w, b, 1.0), bad, D.DeferredLogProbs(hid, w, b, 1.0), y)[0]):
+        assert bool(torch.isnan(loss))
+    if frozen:
+        return
+    up = torch.randn(B, L, generator=gen, device=dev)
+    up[0, 0] = 0.0                                               # nothing asked of a live row
+    gh, gw, gb = torch.autograd.grad((got * up)[~hit].sum() + got[hit].sum(), xs)
+    wh, _, _ = torch.autograd.grad((want * up)[~hit].sum() + want[hit].sum(), xs)
+    assert torch.equal(torch.isnan(gh).any(-1), hit) and torch.isnan(gh).all(-1)[hit].all()
+    assert torch.equal(gh[~hit], wh[~hit])
+    assert bool(torch.isnan(gw).all()) and bool(torch.isnan(gb).all())
+    sums = D.DeferredLogProbs(hid, w, b, 1.0)                    # the sum alone, as a training step asks for it
+    gh, gw, gb = torch.autograd.grad(criterions.NLLEntropy(ignore, None)(sums, bad), xs)
+    assert torch.equal(torch.isnan(gh).all(-1), hit) and torch.equal(torch.isnan(gh).any(-1), hit) and bool(torch.isnan(gw).all())
+
+
+@pytest.mark.parametrize("H,V", PATHS)
+def test_nothing_of_a_bad_batch_stays(dev, H, V):
+    """The NaN of one batch's gradients does not reach the next batch's through a workspace."""
+    from pevae_amd import criterions
+    from pevae_amd.enc2dec import decoders as D
+    gen = torch.Generator(device=dev).manual_seed(33)
+    B, L = 9, 29
+    xs = [(torch.randn(*s, generator=gen, device=dev) * 0.3).requires_grad_() for s in ((B, L, H), (V, H), (V,))]
+    y = torch.randint(1, V, (B, L), generator=gen, device=dev)
+    bad = y.clone()
+    bad[:, 4], y[:, 7:11] = V + 3, 0
+    old, adv = torch.randn(B, L, generator=gen, device=dev) - 7, torch.randn(B, generator=gen, device=dev)
+
+    def grads(labels):
+        out = D.DeferredLogProbs(*xs, 1.0)
+        loss = criterions.NLLEntropy(0, None)(out, labels) + criterions.ClippedPolicyLoss(0, None)(out, labels, old, adv)[0]
+        more = criterions.ClippedPolicyLoss(0, None, ent_coef=0.1)(out, labels, old, adv)[0]
+        return torch.autograd.grad(loss, xs) + torch.autograd.grad(more, xs)
+
+    want = grads(y)
+    assert all(bool(torch.isnan(g).any()) for g in grads(bad))
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(grads(y), want))
