@@ -692,6 +692,27 @@ def grad_sink(param, shape=None):
     return None
 
 
+def ordered_sink(param, shape):
+    """grad_sink() for the nodes of the vocabulary projection that compute its gradient by themselves.  In a backward pass with
+    side work the fused vocabulary node accumulates into that gradient beside the recurrences, on the second side stream, and
+    the engine adds a gradient that was handed back once the last contributing node has run: with several decoder outputs a range
+    may be in flight beside that addition, and one of the two updates is lost.  So the node adds into the sink itself, behind the
+    side streams' work so far; what is launched there later waits for the current stream.  Outside such a pass (None) the
+    gradient is handed back."""
+    if not ASYNC_WGRAD:
+        return None
+    join_side_work()
+    return grad_sink(param, shape)
+
+
+def _into(sink, grad):
+    """What a node returns for `grad`: None once it is added into its sink, the gradient itself without one."""
+    if sink is None:
+        return grad
+    sink.add_(grad)
+    return None
+
+
 def masked_sum(x, mask=None, ignore=0):
     out = torch.empty(2, dtype=torch.float32, device=x.device)
     _lib.call("pv_masked_sum", _p(x), _p(mask), ignore, x.numel(), _p(out), _stream())
@@ -1223,6 +1244,7 @@ class VocabLogProbDense(torch.autograd.Function):
                   _p(logp), _stream())
         ctx.save_for_backward(h_bf, w_bf, logp)
         ctx.dims = (T, H, V, Hp, ldh, inv_temp)
+        ctx.params = (weight, bias)
         return logp
 
     @staticmethod
@@ -1236,8 +1258,10 @@ class VocabLogProbDense(torch.autograd.Function):
         _lib.call("pv_logsoftmax_bwd_bf16", _p(logp), _p(dlogp.contiguous()), T, V, inv_temp, _p(P), Vp, _p(dbias),
                   _stream())
         PT = transpose_to_bf16(P, T, V, Vp, Tp, out=workspace("vocab_PT", Vp * Tp, BF16, dev)[:V * Tp].view(V, Tp))
-        dH, dW = _vocab_stage2(P, PT, h_bf, ldh, w_bf, T, H, V, Hp, Tp, Vp)
-        return dH, dW, dbias, None
+        sink, sink_b = (ordered_sink(p, s) if need else None
+                        for p, s, need in zip(ctx.params, ((V, H), (V,)), ctx.needs_input_grad[1:3]))
+        dH, dW = _vocab_stage2(P, PT, h_bf, ldh, w_bf, T, H, V, Hp, Tp, Vp, sink)
+        return dH, dW, _into(sink_b, dbias), None
 
 
 # ------------------------------------------------------------------------------------------------------------
@@ -3086,6 +3110,7 @@ class ProjectedLoss(torch.autograd.Function):
         out = run((_p(logits), _ROW_DTYPES[torch.float32], B, L, L * Vp, Vp, V), d, Vp, perm)
         ctx.save_for_backward(h_bf, w_bf, d, perm, live)
         ctx.dims = (B, L, H, V)
+        ctx.params = (weight, bias)
         ctx.mark_non_differentiable(*out[1:])
         return out
 
@@ -3117,11 +3142,12 @@ class ProjectedLoss(torch.autograd.Function):
             _launch(dev, "pv_gemm_bf16_tn_splitk", _p(d), Vp, _p(h_bf), Hp, V, H, Tp, max(1, splits.value),
                     _p(ws) if splits.value > 1 else None, _p(dw), H, 0)
             _launch(dev, "pv_scale_by_f32", _p(dw), dw.numel(), _p(g))
-            dw = dw[:V * H].view(V, H)
+            dw = _into(ordered_sink(ctx.params[0], (V, H)), dw[:V * H].view(V, H))
         if need_b:
             db = torch.empty(V, dtype=torch.float32, device=dev)
             ws = torch.empty(_lib.load().pv_colsum_scaled_ws_bytes(V), dtype=torch.uint8, device=dev)
             _launch(dev, "pv_colsum_scaled_bf16", _p(d), Vp, T, V, _p(g), _p(db), _p(ws))
+            db = _into(ordered_sink(ctx.params[1], (V,)), db)
         return dh, dw, db, None, None, None, None
 
 

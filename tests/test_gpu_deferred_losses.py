@@ -164,3 +164,40 @@ def test_nothing_of_a_bad_batch_stays(dev, H, V):
     want = grads(y)
     assert all(bool(torch.isnan(g).any()) for g in grads(bad))
     assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(grads(y), want))
+
+
+@pytest.mark.parametrize("loss", ["distill", "explore", "dense"])
+@pytest.mark.parametrize("order", [(0, 1), (1, 0), (1, 0, 1), (0, 1, 0)])
+def test_several_decoder_passes_in_one_backward_pass(dev, loss, order):
+    """A loss whose weight gradient is a product of its own, on one decoder output, and the NLL, which accumulates into the same
+    gradient beside the recurrences, on others, in every order: the sum of the gradients of each alone.  Each output's share is
+    computed as it is alone; what is left are the roundings of the fp32 additions, at most one of 2^-24 of the partial sum for
+    each of the V + B L terms of an element: 1e-4 of the largest is granted an output."""
+    from pevae_amd import criterions
+    from pevae_amd.dls_vae import DLSVAE
+    from pevae_amd.enc2dec import decoders as D
+    B, L, H, V = 8, 12, 512, 5003
+    dec = decoder(dev, H, V, L)
+    ids, y, h0, adv = answers(dev, B, L, V)
+    h0 = (h0 * 0.3).expand(1, B, H).contiguous().requires_grad_()
+    t = torch.randn(B, L, V, device=dev).topk(8, -1)
+    with torch.no_grad():
+        old = criterions.token_log_probs(dec(B, ids, h0, mode=D.TEACH_FORCE)[0], y, 0) - 0.1
+    one = {"distill": lambda o: criterions.TopKDistill(0, None)(o, y, t.indices, t.values),
+           "explore": lambda o: criterions.ClippedPolicyLoss(0, None, ent_coef=0.1)(o, y, old, adv)[0],
+           "dense": lambda o: criterions.TopKDistill(0, None)(o.materialize(), y, t.indices, t.values)}[loss]
+    other = lambda o: criterions.NLLEntropy(0, None)(o, y)
+    params = list(dec.parameters()) + [h0]
+
+    def grads(chosen):
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        terms = [f(dec(B, ids, h0, mode=D.TEACH_FORCE)[0]) for f in chosen]
+        DLSVAE._run_backward(lambda: torch.autograd.backward(terms))
+        return [p.grad.clone() for p in params]
+
+    alone = [grads([one]), grads([other])]
+    for _ in range(3):
+        for p, got, *each in zip(params, grads([(one, other)[k] for k in order]), *[alone[k] for k in order]):
+            top = max(float(e.abs().max()) for e in each)
+            assert float((got - sum(each)).abs().max()) <= 1e-4 * len(each) * top
