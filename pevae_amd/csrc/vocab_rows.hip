@@ -1087,6 +1087,11 @@ __global__ __launch_bounds__(256) void preference_bwd_kernel(const int64_t* __re
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
 inline int pieces_of(int dtype, int V) { return V / (dtype == PV_DTYPE_F32 ? 4 : 8); }
+// a launch has fewer than 2^32 threads; the ladders below give a row at most these
+inline long threads_of(int dtype, int V) {
+  const int pieces = pieces_of(dtype, V);
+  return pieces <= 512 ? 64 : pieces <= 1024 ? 128 : pieces <= 2048 ? 256 : pieces <= 4096 ? 512 : 1024;
+}
 int check_rows(const char* who, const void* logits, int dtype, long n0, int n1, long s0, long s1, int V, float inv_temp) {
   PV_REQUIRE(logits && n0 > 0 && n1 > 0 && V > 0, "%s: null logits or an empty size", who);
   PV_REQUIRE(dtype == PV_DTYPE_F32 || dtype == PV_DTYPE_BF16 || dtype == PV_DTYPE_F16, "%s: unknown dtype %d", who, dtype);
@@ -1097,10 +1102,7 @@ int check_rows(const char* who, const void* logits, int dtype, long n0, int n1, 
     pv_set_error("%s: %ld x %d rows of %d words are beyond the limit (%ld rows, 2^24 words)", who, n0, n1, V, kRowsMax);
     return PV_ERR_LIMIT;
   }
-  // a launch has fewer than 2^32 threads; the ladders below give a row at most these
-  const int pieces = pieces_of(dtype, V);
-  const long threads = pieces <= 512 ? 64 : pieces <= 1024 ? 128 : pieces <= 2048 ? 256 : pieces <= 4096 ? 512 : 1024;
-  if (n0 * (long)n1 * threads >= 1L << 32) {
+  if (n0 * (long)n1 * threads_of(dtype, V) >= 1L << 32) {
     pv_set_error("%s: %ld rows of %d words are more than a launch has threads for", who, n0 * (long)n1, V);
     return PV_ERR_LIMIT;
   }
@@ -1113,6 +1115,11 @@ int check_count(const char* who, long n, long limit) {
 }
 Rows make_rows(const void* logits, long n0, int n1, long s0, long s1, int V, const int64_t* labels, int64_t ignore, float c) {
   return {logits, n1, V, n0 * (long)n1, s0, s1, c, (float)((double)c * 1.4426950408889634), labels, ignore, nullptr};
+}
+
+// Answers of one type and vocabulary, whose rows fit a launch together too.
+bool share_a_launch(int dtype_a, const Rows& a, int dtype_b, const Rows& b) {
+  return dtype_a == dtype_b && a.V == b.V && a.T + b.T <= kRowsMax && (a.T + b.T) * threads_of(dtype_a, a.V) < 1L << 32;
 }
 
 // Threads a row of the pass that only reads: a wave for short rows (V = 5003, bf16, 20000 rows: 39 us, 256 threads 49), more
@@ -1485,7 +1492,7 @@ int pv_preference_rows_fwd(const void* logits_c, int dtype_c, long pairs, int Lc
   const Rows r = make_rows(logits_r, pairs, Lr, s0r, s1r, Vr, labels_r, ignore, inv_temp);
   const FwdOut oc = {lp_c, nullptr, nullptr, (float4*)save_c}, orr = {lp_r, nullptr, nullptr, (float4*)save_r};
   hipStream_t st = (hipStream_t)stream;
-  if (dtype_c == dtype_r && Vc == Vr && c.T + r.T <= kRowsMax) {
+  if (share_a_launch(dtype_c, c, dtype_r, r)) {
     rc = dtype_c == PV_DTYPE_F32    ? launch_fwd_pair_typed<F32>(c, r, oc, orr, st)
          : dtype_c == PV_DTYPE_BF16 ? launch_fwd_pair_typed<BF16>(c, r, oc, orr, st)
                                     : launch_fwd_pair_typed<F16>(c, r, oc, orr, st);
@@ -1512,7 +1519,7 @@ int pv_preference_rows_bwd(const void* logits_c, int dtype_c, long pairs, int Lc
   const Grad qc = {(const float4*)save_c, nullptr, nullptr, slope, weight, g, dlogits_c, 0};
   const Grad qr = {(const float4*)save_r, nullptr, nullptr, slope, -weight, g, dlogits_r, 0};
   hipStream_t st = (hipStream_t)stream;
-  if (dlogits_c && dlogits_r && dtype_c == dtype_r && Vc == Vr && c.T + r.T <= kRowsMax)
+  if (dlogits_c && dlogits_r && share_a_launch(dtype_c, c, dtype_r, r))
     return dtype_c == PV_DTYPE_F32    ? launch_grad_pair_typed<F32>(c, r, qc, qr, st)
            : dtype_c == PV_DTYPE_BF16 ? launch_grad_pair_typed<BF16>(c, r, qc, qr, st)
                                       : launch_grad_pair_typed<F16>(c, r, qc, qr, st);

@@ -1,8 +1,8 @@
-"""Losses over rows of a vocabulary softmax in memory where one value could hide another."""
+"""Losses over rows of a vocabulary softmax in memory where one value could hide another, and where two answers share a launch."""
 import pytest
 import torch
 
-from test_gpu_vocab_rows import dev, make  # noqa: F401
+from test_gpu_vocab_rows import EXP, dev, make  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,25 @@ def test_a_zero_advantage_hides_no_nan(dev, kl):
         loss, _ = ops.projected_policy_loss(hid, w, b, t, o, adv, old if kl else None, -7, kl_coef=kl, ent_coef=0.1)
         gh, = torch.autograd.grad(loss, hid)
         assert bool(torch.isnan(loss)) == lost and bool(torch.isnan(gh[1, 2]).all()) == lost and not bool(torch.isnan(gh[0]).any())
+
+
+def test_answers_that_pass_a_launch_only_one_by_one(dev):
+    """Two answers of 2^13 x 1 040 rows, 256 threads a row: 2^31.02 threads each, more than 2^32 together.  All rows but a few are
+    dead and every row of logits is the same one in memory (strides of 0)."""
+    from pevae_amd import ops
+    P, L, V = 1 << 13, 1040, 8203
+    z = make((V,), torch.bfloat16, dev, 410)
+    y = torch.full((P, L), -7, dtype=torch.int64, device=dev)
+    y[0, 0], y[P - 1, L - 1], y[77, 3] = 5, V - 1, 100
+    yr = y.clone()
+    yr[P - 1, L - 1] = 7
+    rows = z.expand(P, L, V)
+    loss, rc, rr = ops.vocab_preference_loss(rows, y, rows, yr, ignore_index=-7, beta=0.3, avg_type=None)
+    lp = torch.log_softmax(z.double(), -1)
+    want_c, want_r = torch.zeros(P, dtype=torch.float64, device=dev), torch.zeros(P, dtype=torch.float64, device=dev)
+    want_c[0], want_c[77], want_c[P - 1] = lp[5], lp[100], lp[V - 1]
+    want_r[0], want_r[77], want_r[P - 1] = lp[5], lp[100], lp[7]
+    for got, want in ((rc, 0.3 * want_c), (rr, 0.3 * want_r)):
+        assert float((got.double() - want).abs().max()) <= EXP * (1 + float(want.abs().max()))
+    total = -torch.nn.functional.logsigmoid(0.3 * (want_c - want_r)).sum()
+    assert abs(float(loss) - float(total)) <= EXP * float(total)
