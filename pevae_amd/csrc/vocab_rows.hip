@@ -1069,7 +1069,7 @@ __global__ __launch_bounds__(256) void preference_kernel(Answers c, Answers r, i
   const float up = x >= 0.f ? l : l - x, down = x >= 0.f ? l + x : l;   // -ln sig(x), -ln sig(-x)
   const float small = q / (1.f + q), large = 1.f / (1.f + q);           // sig(-|x|), sig(|x|)
   const float sig = x >= 0.f ? large : small, gis = x >= 0.f ? small : large;
-  float loss = (1.f - smooth) * up;
+  float loss = smooth != 1.f ? (1.f - smooth) * up : 0.f;               // up and down may be infinite
   if (smooth != 0.f) loss += smooth * down;
   rowout[b] = make_float4(x != x ? x : loss, 0.f, 0.f, 0.f);
   slope[b] = beta * (smooth * sig - (1.f - smooth) * gis);

@@ -72,3 +72,20 @@ def test_answers_that_pass_a_launch_only_one_by_one(dev):
         assert float((got.double() - want).abs().max()) <= EXP * (1 + float(want.abs().max()))
     total = -torch.nn.functional.logsigmoid(0.3 * (want_c - want_r)).sum()
     assert abs(float(loss) - float(total)) <= EXP * float(total)
+
+
+def test_preference_of_an_impossible_answer(dev):
+    """Rewards of -inf and inf: the term that does not count (label_smoothing 0 or 1) adds nothing, the other one 0 or inf."""
+    from pevae_amd import ops
+    y = torch.ones(1, 1, dtype=torch.int64, device=dev)
+    zero = torch.zeros(1, 1, device=dev)
+    none = torch.full((1, 1), -INF, device=dev)
+    for c, r, smooth, want in ((none, zero, 0.0, INF), (none, zero, 1.0, 0.0), (zero, none, 0.0, 0.0), (zero, none, 1.0, INF),
+                               (none, zero, 0.25, INF), (zero, none, 0.25, INF)):
+        c, r = c.clone().requires_grad_(), r.clone().requires_grad_()
+        loss, _, _ = ops.preference_loss(c, y, r, y, beta=0.5, label_smoothing=smooth)
+        assert float(loss) == want, (smooth, float(loss))
+        dc, dr = torch.autograd.grad(loss, [c, r])
+        sig = 0.0 if float(c) < 0 else 1.0              # of the difference of the rewards
+        slope = 0.5 * (smooth * sig - (1 - smooth) * (1 - sig))
+        assert float(dc) == slope and float(dr) == -slope
