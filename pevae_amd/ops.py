@@ -3169,6 +3169,11 @@ def _projection(hid, weight, bias):
     return hid.shape[:2]
 
 
+def _no_rows(hid, weight, bias):
+    """The loss of an empty batch: 0, with a zero gradient of every operand."""
+    return hid.sum() + weight[:0].sum() + bias[:0].sum()
+
+
 def _projected(hid, weight, bias, labels, ignore, run):
     want = torch.is_grad_enabled() and (hid.requires_grad or weight.requires_grad or bias.requires_grad)
     with torch.cuda.device(hid.device):
@@ -3185,7 +3190,7 @@ def projected_distill_topk(hid, proj_weight, proj_bias, teacher_ids, teacher_log
     w, word = _avg(avg_type, weight, shape[0])
     dev = _same_device(hid, proj_weight, proj_bias, ids, tl, labels)
     if ids.numel() == 0:
-        return hid.sum() * 0.0
+        return _no_rows(hid, proj_weight, proj_bias)
     ignore, K, T = _NO_INDEX if ignore_index is None else int(ignore_index), ids.shape[-1], shape[0] * shape[1]
 
     def run(rows, d, ld, perm):
@@ -3211,7 +3216,7 @@ def projected_policy_loss(hid, proj_weight, proj_bias, tokens, old_logp, advanta
     dev = _same_device(hid, proj_weight, proj_bias, tokens, old, adv, ref)
     T = tokens.numel()
     if T == 0:
-        return hid.sum() * 0.0, torch.zeros(4, dtype=torch.float32, device=dev)
+        return _no_rows(hid, proj_weight, proj_bias), torch.zeros(4, dtype=torch.float32, device=dev)
     ignore = _NO_INDEX if ignore_index is None else int(ignore_index)
 
     def run(rows, d, ld, perm):

@@ -201,3 +201,20 @@ def test_several_decoder_passes_in_one_backward_pass(dev, loss, order):
         for p, got, *each in zip(params, grads([(one, other)[k] for k in order]), *[alone[k] for k in order]):
             top = max(float(e.abs().max()) for e in each)
             assert float((got - sum(each)).abs().max()) <= 1e-4 * len(each) * top
+
+
+def test_empty_projections(dev):
+    """Without a row every operand has a zero gradient, whichever of them asks."""
+    from pevae_amd import ops
+    V, H = 9, 16
+    w, b = torch.randn(V, H, device=dev), torch.randn(V, device=dev)
+    for shape in ((0, 4, H), (4, 0, H)):
+        y = torch.zeros(shape[:2], dtype=torch.int64, device=dev)
+        f = torch.zeros(shape[:2], device=dev)
+        for asks in ((True, True, True), (False, True, True), (False, False, True), (True, False, False)):
+            xs = [x.detach().clone().requires_grad_(a) for x, a in zip((torch.zeros(shape, device=dev), w, b), asks)]
+            for loss in (ops.projected_distill_topk(*xs, y[..., None], f[..., None]), ops.projected_policy_loss(*xs, y, f, f)[0]):
+                assert float(loss) == 0.0
+                wanted = [x for x in xs if x.requires_grad]
+                for x, g in zip(wanted, torch.autograd.grad(loss, wanted)):
+                    assert g.shape == x.shape and int(torch.count_nonzero(g)) == 0
