@@ -15,6 +15,9 @@ typedef uint16_t bf16_t;   // raw bf16 bits in memory
 #define PV_ERR_TIMEOUT -4  // a bounded in-kernel spin gave up (persistent GRU)
 
 void pv_set_error(const char* fmt, ...);
+// Clears `bytes` (a multiple of 4) by a kernel of its own: callers capture these launches into HIP graphs, where a memset node has
+// left other values from the second replay on.
+int pv_clear(void* p, size_t bytes, hipStream_t stream);
 
 #define PV_REQUIRE(cond, ...)                 \
   do {                                        \
@@ -31,6 +34,12 @@ void pv_set_error(const char* fmt, ...);
       pv_set_error("%s: launch failed: %s", name, hipGetErrorString(e__)); \
       return PV_ERR_HIP;                                                  \
     }                                                                     \
+  } while (0)
+
+#define PV_CLEAR(p, bytes, stream)                     \
+  do {                                                 \
+    const int rc__ = pv_clear(p, bytes, stream);       \
+    if (rc__ != PV_OK) return rc__;                    \
   } while (0)
 
 #define PV_HIP(call)                                                      \

@@ -825,7 +825,7 @@ int pv_pick_nll_bwd(const float* dout, const int64_t* target, int64_t ignore, in
                     void* stream) {
   PV_REQUIRE(dout && target && dlogp && T > 0 && V > 0, "pv_pick_nll_bwd: bad argument");
   hipStream_t st = (hipStream_t)stream;
-  PV_HIP(hipMemsetAsync(dlogp, 0, (size_t)T * V * sizeof(float), st));
+  PV_CLEAR(dlogp, (size_t)T * V * sizeof(float), st);
   hipLaunchKernelGGL(pick_nll_bwd_kernel, dim3(cdiv(T, 256)), dim3(256), 0, st, dout, target, ignore, T, V, dlogp);
   PV_LAUNCH_CHECK("pick_nll_bwd_kernel");
   return PV_OK;

@@ -359,7 +359,7 @@ int pv_embedding_bwd_sorted(const float* grad_rows, int ldg, int n, long num_row
   PV_REQUIRE(n >= 0 && D > 0 && ldg >= D, "pv_embedding_bwd_sorted: bad sizes");
   PV_REQUIRE(ws_bytes >= pv_embedding_bwd_ws_bytes(n, D), "pv_embedding_bwd_sorted: workspace too small");
   hipStream_t st = (hipStream_t)stream;
-  if (!accumulate) PV_HIP(hipMemsetAsync(dtable, 0, (size_t)num_rows * D * sizeof(float), st));
+  if (!accumulate) PV_CLEAR(dtable, (size_t)num_rows * D * sizeof(float), st);
   if (n == 0) return PV_OK;
   const size_t a = round_up(n, 64) * sizeof(int);
   char* ws = (char*)workspace;

@@ -1266,7 +1266,7 @@ int pv_vocab_nll_bwd_prob(const void* h, int ldh, const void* W, int ldw, const 
              "pv_vocab_nll_bwd_prob: need ldp >= %d and ldpt >= %d (multiples of 8)", Vpad, Tpad);
   PV_REQUIRE(((uintptr_t)P & 15) == 0 && ((uintptr_t)PT & 15) == 0, "pv_vocab_nll_bwd_prob: P/PT must be 16-byte aligned");
   hipStream_t st = (hipStream_t)stream;
-  if (live_rows) PV_HIP(hipMemsetAsync(dbias_part, 0, (size_t)(Tpad / 64) * ldp * sizeof(float), st));   // skipped tiles
+  if (live_rows) PV_CLEAR(dbias_part, (size_t)(Tpad / 64) * ldp * sizeof(float), st);   // skipped tiles
   GemmArgs g{(const bf16_t*)h, (const bf16_t*)W, T, V, H, ldh, ldw, 1, 0, live_rows, nullptr};
   EpiProb e{bias, target, lse, gscale, (bf16_t*)P, (bf16_t*)PT, dbias_part, T, V, Tpad, Vpad, ldp, ldpt, inv_temp};
   rc = big_tile(T, V, H) ? launch<decltype(e), 4>(g, e, st, "pv_vocab_nll_bwd_prob") : launch(g, e, st, "pv_vocab_nll_bwd_prob");

@@ -768,7 +768,7 @@ static int decode_impl(const float* gx_table, const float* gx_const, const void*
   static const int dbg = getenv("PV_DECODE_DBG") ? atoi(getenv("PV_DECODE_DBG")) : 0;
   a.dbg = dbg;
   hipStream_t st = (hipStream_t)stream;
-  if (p.Hk != p.S * UNITS) PV_HIP(hipMemsetAsync(a.hb, 0, p.hb_bytes, st));   // padding columns no slice ever writes
+  if (p.Hk != p.S * UNITS) PV_CLEAR(a.hb, p.hb_bytes, st);   // padding columns no slice ever writes
   const int n0 = p.Bpad * p.Hk > (int)(SYNC_BYTES / 4) ? p.Bpad * p.Hk : (int)(SYNC_BYTES / 4);
   hipLaunchKernelGGL(decode_init_kernel, dim3(cdiv(n0, 256)), dim3(256), 0, st, h0, B, H, p.Hk, p.Bpad, a.hb, (u32*)ws,
                      (int)(SYNC_BYTES / 4));

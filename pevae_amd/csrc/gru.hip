@@ -1017,10 +1017,10 @@ int rnn_fwd(int ngt, const float* xprojT, long ldx, const void* whh_bf16, const 
   const int xmap = xcd_map(G, S, cap), grid = xmap ? 8 * cdiv(G, 8) * S : G * S;
   u32* err = (u32*)sync + NG;
   u32* counters = err + 1;
-  if (Hk != H || Bpad != B) PV_HIP(hipMemsetAsync(hseq_bf16, 0, (size_t)(L + 1) * Bpad * Hk * 2, st));
+  if (Hk != H || Bpad != B) PV_CLEAR(hseq_bf16, (size_t)(L + 1) * Bpad * Hk * 2, st);
   if (Bpad != B) {
-    PV_HIP(hipMemsetAsync(hall, 0, (size_t)Bpad * H * sizeof(float), st));      // slot 0 rows >= B are read as states
-    if (ngt == 4) PV_HIP(hipMemsetAsync(call, 0, (size_t)Bpad * H * sizeof(float), st));
+    PV_CLEAR(hall, (size_t)Bpad * H * sizeof(float), st);      // slot 0 rows >= B are read as states
+    if (ngt == 4) PV_CLEAR(call, (size_t)Bpad * H * sizeof(float), st);
   }
   const int sync_words = (int)(pv_gru_sync_bytes(B) / sizeof(u32));       // the grid must cover them too (small B * H)
   hipLaunchKernelGGL(gru_pack_h0_kernel, dim3(cdiv(B * H > sync_words ? B * H : sync_words, 256)), dim3(256), 0, st, h0, B, H, Hk, (bf16_t*)hseq_bf16, hn, hall,
@@ -1112,9 +1112,9 @@ int rnn_bwd(int ngt, const float* dout, long dout_sb, long dout_st, const float*
     PV_LAUNCH_CHECK("rnn_bwd_zero_kernel");
   }
   if (K3 != ngt * H || Bpad != B) {
-    if (dgi_bf16) PV_HIP(hipMemsetAsync(dgi_bf16, 0, (size_t)L * Bpad * K3 * 2, st));
-    PV_HIP(hipMemsetAsync(dgh_bf16, 0, (size_t)L * Bpad * K3 * 2, st));
-    if (dgx_bf16) PV_HIP(hipMemsetAsync(dgx_bf16, 0, (size_t)L * Bpad * K3 * 2, st));
+    if (dgi_bf16) PV_CLEAR(dgi_bf16, (size_t)L * Bpad * K3 * 2, st);
+    PV_CLEAR(dgh_bf16, (size_t)L * Bpad * K3 * 2, st);
+    if (dgx_bf16) PV_CLEAR(dgx_bf16, (size_t)L * Bpad * K3 * 2, st);
   }
   GruBwdArgs a{dout, dout_sb, dout_st, dhn, gsaveT, hall, (const bf16_t*)whhT_bf16, (bf16_t*)dgi_bf16,
                (bf16_t*)dgh_bf16, ngt == 4 ? dc0 : dh0, call, dcn, dh0, dbias_part, counters, err, L, B, H, K3, Bpad,

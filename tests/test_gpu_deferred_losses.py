@@ -218,3 +218,88 @@ def test_empty_projections(dev):
                 wanted = [x for x in xs if x.requires_grad]
                 for x, g in zip(wanted, torch.autograd.grad(loss, wanted)):
                     assert g.shape == x.shape and int(torch.count_nonzero(g)) == 0
+
+
+def test_policy_loss_behind_the_tile_kernels_captured(dev):
+    """Forward and backward of a policy step at a hidden size of the tile kernels, replayed with eager work and changed inputs and
+    labels between: the live rows, and with them the tiles that are skipped, differ from replay to replay."""
+    from pevae_amd import criterions
+    from pevae_amd.enc2dec import decoders as D
+    B, L, H, V = 40, 7, 64, 1003
+    gen = torch.Generator(device=dev).manual_seed(50)
+    params = [torch.randn(*s, generator=gen, device=dev) * 0.3 for s in ((B, L, H), (V, H), (V,))]
+    y0 = torch.randint(1, V, (B, L), generator=gen, device=dev)
+    old, adv = torch.randn(B, L, generator=gen, device=dev) - 7, torch.randn(B, generator=gen, device=dev)
+    policy = criterions.ClippedPolicyLoss(0, None)
+
+    def step(xs, y):
+        loss, stats = policy(D.DeferredLogProbs(*xs, 1.0), y, old, adv)
+        return [loss.detach(), stats] + list(torch.autograd.grad(loss, xs))
+
+    held, y = [x.clone().requires_grad_() for x in params], y0.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(held, y)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(held, y)
+    for turn in range(5):
+        keep = torch.rand(B, L, generator=gen, device=dev) < (0.9, 0.1, 0.5, 0.02, 1.0)[turn]
+        with torch.no_grad():
+            y.copy_(torch.where(keep, y0, torch.zeros_like(y0)))
+            for x, v in zip(held, params):
+                x.copy_(v * (1.0 + 0.1 * turn))
+        want = step([(v * (1.0 + 0.1 * turn)).requires_grad_() for v in params], y.clone())
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
+@pytest.mark.parametrize("cell", ["gru", "lstm"])
+@pytest.mark.parametrize("B,H", [(5, 48), (7, 64), (16, 80)])
+def test_decoder_step_with_padded_states_captured(dev, cell, B, H):
+    """A policy step through the decoder, batch and hidden sizes that the recurrence pads, replayed with eager work and changed
+    weights, inputs and labels between."""
+    import copy
+    from pevae_amd import criterions
+    from pevae_amd.enc2dec import decoders as D
+    torch.manual_seed(9)
+    L, E, V = 7, 24, 211
+    held = D.DecoderRNN(V, L, E, H, 1, 2, 3, rnn_cell=cell, embedding=torch.nn.Embedding(V, E, padding_idx=0)).to(dev)
+    eager = copy.deepcopy(held)
+    ids, y, _, adv = answers(dev, B, L, V)
+    state = torch.randn(2, 1, B, H, device=dev) * 0.3
+    old = torch.randn(B, L, device=dev) - 5
+    policy = criterions.ClippedPolicyLoss(0, None)
+
+    def step(dec):
+        h0 = (state[0], state[1]) if cell == "lstm" else state[0]
+        loss, stats = policy(dec(B, ids, h0, mode=D.TEACH_FORCE)[0], y, old, adv)
+        return [loss.detach(), stats] + list(torch.autograd.grad(loss, list(dec.parameters())))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(held)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(held)
+    for turn in range(5):
+        gen = torch.Generator(device=dev).manual_seed(60 + turn)
+        with torch.no_grad():
+            ids.copy_(torch.randint(4, V, (B, L), generator=gen, device=dev))
+            y[:, :-1] = ids[:, 1:]
+            y[1, turn:] = 0
+            state.copy_(torch.randn(2, 1, B, H, generator=gen, device=dev) * 0.3)
+            for p, q in zip(held.parameters(), eager.parameters()):
+                q.mul_(1.05)
+                p.copy_(q)
+        want = step(eager)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
