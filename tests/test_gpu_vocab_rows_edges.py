@@ -1,8 +1,9 @@
-"""Losses over rows of a vocabulary softmax in memory where one value could hide another, and where two answers share a launch."""
+"""Losses over rows of a vocabulary softmax in memory: where one value could hide another, where two answers share a launch, and
+their gradients against differences along the gradient itself."""
 import pytest
 import torch
 
-from test_gpu_vocab_rows import EXP, dev, make  # noqa: F401
+from test_gpu_vocab_rows import EXP, dev, labels_of, make  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,43 @@ def test_preference_of_an_impossible_answer(dev):
         sig = 0.0 if float(c) < 0 else 1.0              # of the difference of the rewards
         slope = 0.5 * (smooth * sig - (1 - smooth) * (1 - sig))
         assert float(dc) == slope and float(dr) == -slope
+
+
+@pytest.mark.parametrize("kind", ["logp", "distill", "policy", "preference"])
+def test_gradients_against_differences_along_them(dev, kind):
+    """Along w = d / |d| the derivative is |d|.  Central differences at h and 2 h, combined so that the h^2 term cancels, leave
+    h^4 / 30 of the fifth derivative along w; each loss is off by EXP (1 + |loss|) at most, which enters
+    (4 / 3 + 1 / 6) / h times.  Fifth derivatives: those of ln sum e^z along a unit direction are cumulants of a variable of
+    range R <= sqrt 2, |k5| = |m5 - 10 m2 m3| <= R^5 / 4 + 10 (R^2 / 4) (R^3 / 4) < 5 (with |m_n| <= R^n / 4); the entropy adds a
+    factor of z (below 10 here); a ratio e^lp of about 5 has e^lp times the complete Bell polynomial of such derivatives, below
+    52 R^5 = 300, over ten live tokens.  120 covers each.  The ratios of the policy loss stay on their side of the clip range."""
+    from pevae_amd import ops
+    B, L, V, K, h = 3, 4, 257, 9, 0.05
+    z = make((B, L, V), torch.float32, dev, 420, 1.0)
+    y = labels_of((B, L), V, dev, 421, 0.2)
+    t = make((B, L, V), torch.float32, dev, 422).topk(K, -1)
+    lp0 = ops.token_logprobs(z, y, ignore_index=-7)
+    old = lp0 - torch.where(torch.arange(B * L, device=dev).view(B, L) % 2 == 0, 0.05, 1.5)     # ratios of 1.05 and 4.5; range 0.5 to 1.5
+    adv = torch.tensor([1.0, -0.7, 0.4], device=dev)
+
+    def loss_of(x):
+        if kind == "logp":
+            lp, H = ops.token_logprobs(x, y, ignore_index=-7, inv_temp=0.9, entropy=True)
+            return (lp * old).sum() / 12 + H.sum() / 12
+        if kind == "distill":
+            return ops.distill_topk(x, t.indices, t.values, y, -7, 1.5, avg_type="word")
+        if kind == "policy":
+            return ops.vocab_policy_loss(x, y, old, adv, lp0 - 0.1, -7, clip=0.5, kl_coef=0.1, ent_coef=0.05)[0]
+        return ops.vocab_preference_loss(x, y, x.flip(0), y.flip(0), lp0, lp0.flip(0) - 0.3, -7, beta=1.0)[0]
+
+    x = z.clone().requires_grad_()
+    loss = loss_of(x)
+    d, = torch.autograd.grad(loss, x)
+    size = float(d.double().norm())
+    way = (d.double() / size).float()
+    with torch.no_grad():
+        at = {s: float(loss_of(z + s * h * way)) for s in (-2, -1, 1, 2)}
+    diff = (4 * (at[1] - at[-1]) / 2 - (at[2] - at[-2]) / 4) / (3 * h)
+    tol = h ** 4 / 30 * 120 + 1.5 * EXP * (1 + abs(float(loss))) / h
+    assert abs(diff - size) <= tol
+    assert tol <= 0.1 * size                # a gradient of 0, of the other sign, or a tenth off would not pass
