@@ -1122,10 +1122,18 @@ bool share_a_launch(int dtype_a, const Rows& a, int dtype_b, const Rows& b) {
   return dtype_a == dtype_b && a.V == b.V && a.T + b.T <= kRowsMax && (a.T + b.T) * threads_of(dtype_a, a.V) < 1L << 32;
 }
 
-// Threads a row of the pass that only reads: a wave for short rows (V = 5003, bf16, 20000 rows: 39 us, 256 threads 49), more
-// for longer ones (V = 20004, bf16, 12800 rows, half of them dead: 256 threads 49 us, 64 58, 1024 82; V = 64001, fp32, 3000 rows:
-// 1024 threads 125 us, 256 132; one row of V = 131071, fp32: 1024 threads 10.4 us, 256 17.5).  Splitting one row over workgroups
-// and joining the parts in a second launch took 9.4 us there, and more than one launch everywhere else.
+// Threads a row of the pass that only reads: fewer for short rows, whose workgroups cost more than their words, and for many
+// rows.  us at the borders, the side in front and the one behind (log-probabilities, half of the 12800 rows and none of the 400
+// dead, bf16 / fp32):
+//     256 pieces  T = 12800: 64  9.7 / 8.0, 256 14.9 / 12.9                   T = 400:  64 6.2 / 6.4, 256  6.5 / 6.1
+//    1000         T = 12800: 64 27.0 / 22.7, 256 23.6 / 20.6 (512 pieces: 64 15.5 / 12.5, 256 17.9 / 15.3)
+//    4096         T = 12800: 256 76.7 / 74.5, 512 73.1 / 72.8                 T = 400: 256 9.0 / 7.5, 1024 9.3 / 8.2
+//    6100         T = 12800: 512 112 / 110, 1024 129 / 109; T = 600: 512 12.3 / 10.1, 1024 10.7 / 9.2
+//    8000         T = 12800: 512 144 / 141, 1024 152 / 136; T = 600: 512 15.0 / 12.1, 1024 12.4 / 10.6
+//   12000         T = 12800: 512 216 / 207, 1024 204 / 197
+// and one row of V = 131071, fp32: 1024 10.4, 256 17.5.  Few rows take more threads each, which they leave idle otherwise (1000
+// pieces, T = 400: 64 7.1, 256 6.6).  Splitting one row over workgroups and joining the parts in a second launch took 9.4 us for
+// that row, and more than one launch everywhere else.
 template <class E, int HEAD, bool ENT>
 int launch_fwd_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, hipStream_t st) {
   const int pieces = a.V / E::N;
@@ -1164,11 +1172,23 @@ int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, co
 }
 
 // The one-pass kernel takes the fewest threads that can hold a row: fewer threads with more pieces each keep more rows of a CU
-// in flight.  Rates of live reads and writes (policy loss, TB/s): V = 1009, bf16: 64 x 4 3.1, 128 x 4 2.5; V = 5003, bf16:
-// 128 x 8 4.0, 256 x 4 3.7, 512 x 2 2.7; V = 20004, bf16: 512 x 6 4.8, 1024 x 4 3.8; V = 20004, fp32: 1024 x 6 5.3, 512 x 10 4.9.
-// Beyond 8 pieces a thread of a full CU the threads get more registers and a CU fewer rows: V = 80000, bf16: 512 x 20 (two
-// rows) 4.8, 1024 x 12 (one row) 4.2; V = 131071, bf16: 1024 x 16 3.9, which still beats two passes over memory (2.4).  Keeping
-// part of such rows in shared memory to hold two of them gained nothing (512 x 23 + 9: 3.6, its registers spill).
+// in flight.  TB/s of live reads and of writes at each border, the rung in front of it and the next ones (policy loss, half of
+// the rows dead, odd numbers of words, bf16 / fp32):
+//     256 pieces   64 x 4 3.88 / 3.93     128 x 8 3.74 / 4.06     256 x 8 2.84 / 3.22
+//     512          64 x 8 3.95 / 4.05     128 x 8 4.08 / 4.13     256 x 8 4.13 / 4.30
+//    1024         128 x 8 3.89 / 4.01     256 x 8 4.13 / 4.22     512 x 8 3.98 / 4.38
+//    2048         256 x 8 4.10 / 4.28     512 x 8 4.40 / 4.37    1024 x 8 3.94 / 4.45
+//    4000         512 x 8 4.19 / 4.35    1024 x 6 4.45 / 4.63
+//    6144        1024 x 6 4.34 / 4.53    512 x 20 4.30 / 4.48
+//    8000        1024 x 8 4.20 / 4.40    512 x 20 4.15 / 4.39   1024 x 12 3.72 / 4.54
+//   10000        512 x 20 3.96 / 4.20   1024 x 12 3.73 / 4.40
+// The upper end of a rung would gain 0 to 11 % by the next one, its lower end loses more (500 pieces: 512 x 6 2.8 / 3.3).
+// At one number of threads, pieces that a row does not fill cost registers, and with them rows of a CU (two full rungs against
+// one that the row fits): 64 x 8 for 4 up to 20 %, 512 x 8 for 6 7 to 9 % with a bf16 gradient of fp32 rows, 1024 x 8 for 6 3 to
+// 7 % there and in the distillation of 16-bit rows, 1024 x 16 for 12 3 to 5 % in their policy loss, 20 for 16 1 to 3 %.  (64 x 2
+// and 256 x 6 gave 1 and 2 % at most and are not kept.)  Beyond 10 240 pieces a CU holds one row, which still beats two passes over
+// memory (V = 131071, bf16: 3.9 against 2.4).  Keeping part of such rows in shared memory to hold two of them gained nothing
+// (512 x 23 + 9: 3.6, its registers spill).
 constexpr int kOncePieces = 1024 * 20;            // of a row that the one-pass kernel holds
 template <class E, class O, int HEAD>
 int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const Scale& sc, const FwdOut& o, void* grad, long ldg,
@@ -1183,11 +1203,9 @@ int launch_once_typed(const Rows& a, const Policy& hp, const Distill& hd, const 
     PV_LAUNCH_CHECK("rows_once_kernel");                                                                        \
     return PV_OK;                                                                                               \
   }
-  PV_ONCE(64, 2, 8)
   PV_ONCE(64, 4, 8)
   PV_ONCE(64, 8, 6)
   PV_ONCE(128, 8, 7)
-  PV_ONCE(256, 6, 8)
   PV_ONCE(256, 8, 7)
   PV_ONCE(512, 6, 8)
   PV_ONCE(512, 8, 6)
@@ -1217,6 +1235,12 @@ int check_gradient(const char* who, int dtype, int V, const void* save, const vo
   return PV_OK;
 }
 
+// The gradient pass: a wave a row for short ones, 256 threads for 1024 pieces of a longer one.  us, half of the rows dead, the
+// shapes of 0.3 GB or 60000 rows (bf16 / fp32): 100 pieces 64 33 / 29, 256 80 / 75; 200 49 / 47, 95 / 89; 300 96 / 95, 110 / 106;
+// 512 95 / 95, 97 / 95; 1100 102 / 99, 106 / 103, but with 600 rows 8.6 / 7.5, 6.7 / 6.2.  Shares of 512 and 2048 pieces: 2500
+// pieces 102 / 99, 107 / 103, of 1024 103 / 100; 16384 97 / 95, 96 / 95, of 1024 94 / 92.  2048 workgroups: a launch that finds the
+// gradient ready ends in 5 us with 512 as well, and one that does not takes 97 to 141 us with 512 or 1024, 85 with 2048 (V = 5003,
+// bf16, 20000 rows).
 template <class E, int HEAD>
 int launch_grad_typed(const Rows& a, const Distill& hd, const Grad& q, hipStream_t st) {
   const int pieces = a.V / E::N;
