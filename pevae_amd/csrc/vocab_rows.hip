@@ -1186,8 +1186,9 @@ int launch_fwd(int dtype, const Rows& a, const Policy& hp, const Distill& hd, co
 // At one number of threads, pieces that a row does not fill cost registers, and with them rows of a CU (two full rungs against
 // one that the row fits): 64 x 8 for 4 up to 20 %, 512 x 8 for 6 7 to 9 % with a bf16 gradient of fp32 rows, 1024 x 8 for 6 3 to
 // 7 % there and in the distillation of 16-bit rows, 1024 x 16 for 12 3 to 5 % in their policy loss, 20 for 16 1 to 3 %.  (64 x 2
-// and 256 x 6 gave 1 and 2 % at most and are not kept.)  Beyond 10 240 pieces a CU holds one row, which still beats two passes over
-// memory (V = 131071, bf16: 3.9 against 2.4).  Keeping part of such rows in shared memory to hold two of them gained nothing
+// and 256 x 6 gave 1 and 2 % at most and are not kept.)  Beyond 10 240 pieces a CU holds one row,
+// which still beats two passes over memory: at the last border 3.7 / 4.4 TB/s (distillation, K = 64) and 3.6 / 4.35 (policy), behind
+// it 3.3 / 3.4 and 3.0 / 3.2.  Keeping part of such rows in shared memory to hold two of them gained nothing
 // (512 x 23 + 9: 3.6, its registers spill).
 constexpr int kOncePieces = 1024 * 20;            // of a row that the one-pass kernel holds
 template <class E, class O, int HEAD>

@@ -3081,7 +3081,9 @@ def policy_loss(logp, tokens, old_logp, advantages, ref_logp=None, ignore_index=
 class ProjectedLoss(torch.autograd.Function):
     """A loss over vocabulary rows behind the projection hid W^T + b, with the gradients of all three: the logits live in fp32
     between two kernels, their gradient in bf16 as the operand of the two products that follow (the projection's own operands
-    are bf16 too).  Rows that are dead by `labels` go last and are not multiplied.
+    are bf16 too).  Rows that are dead by `labels` go last where a gradient is wanted: the logits' and the states' products stop
+    in front of them, the weight gradient's and the bias's sum meet zeros there.  Without a gradient every row is multiplied, and
+    the dead ones are not read.
     run(row arguments, gradient or None, its row length, order of the rows or None) -> (loss, further outputs): the C call."""
 
     @staticmethod

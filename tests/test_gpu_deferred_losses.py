@@ -303,3 +303,25 @@ def test_decoder_step_with_padded_states_captured(dev, cell, B, H):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
+@pytest.mark.parametrize("H,V", PATHS)
+def test_the_first_ratio_is_one(dev, H, V):
+    """Scores made under no_grad are, bit for bit, the log-probabilities that the loss computes: the ratio of the first on-policy
+    step is 1, and its gradient that of minus the advantage times the log-probability."""
+    from pevae_amd import criterions, ops
+    from pevae_amd.enc2dec import decoders as D
+    B, L = 5, 6
+    dec = decoder(dev, H, V)
+    ids, y, h0, adv = answers(dev, B, L, V)
+    out = dec(B, ids, (h0 * 0.3).expand(1, B, H).contiguous(), mode=D.TEACH_FORCE)[0]
+    with torch.no_grad():
+        old = criterions.token_log_probs(out, y, 0)
+    lp = criterions.token_log_probs(out, y, 0)
+    assert lp.requires_grad and torch.equal(lp, old)
+    loss, stats = criterions.ClippedPolicyLoss(0, None, avg_type=None)(out, y, old, adv)
+    live = (y != 0).double()
+    assert abs(float(loss) + float((live * adv.double()[:, None]).sum())) <= 2.0 ** -24 * float((live * adv.double().abs()[:, None]).sum())
+    d, = torch.autograd.grad(ops.policy_loss(lp, y, old, adv, ignore_index=0, avg_type=None)[0], lp)
+    assert torch.equal(d, torch.where(y != 0, -adv[:, None].expand(B, L), torch.zeros(B, L, device=dev)))
+    assert float(stats[2]) == 0.0
