@@ -68,8 +68,8 @@ int pv_gemm_bf16_tn_splitk(const void* A, int lda, const void* B, int ldb, int M
 /* ---- fused vocabulary projection + log-softmax + NLL -----------------------------------------------------
  * Forward: logits = (h W^T + bias) * inv_temp are produced tile-wise by the MFMA GEMM and reduced on the fly
  * to per-token lse[t] and nll[t] = lse - logit[target] (0 where target == ignore_index, NaN where any other is
- * outside [0, V)); the [T,V] log-prob tensor is never written.  Replaces decoders.py:191-193 (Linear + /temperature + log_softmax) fused with
- * criterions.py:55-64 (NLLLoss sum) and criterions.py:133-138 (Perplexity's token mean).
+ * outside [0, V)); the [T,V] log-prob tensor is never written.  Replaces decoders.py:191-193 (Linear + /temperature +
+ * log_softmax) fused with criterions.py:55-64 (NLLLoss sum) and criterions.py:133-138 (Perplexity's token mean).
  * h [T][ldh] bf16, W [V][ldw] bf16, H % 64 == 0. */
 size_t pv_vocab_nll_fwd_ws_bytes(int T, int V);
 int pv_vocab_nll_fwd(const void* h, int ldh, const void* W, int ldw, const float* bias, const int64_t* target,

@@ -88,6 +88,8 @@ class DeferredLogProbs(object):
         res = make()
         if keep(res):
             self._nll_cache[on, key] = res
+            if on:
+                self._nll_cache.pop((False, key), None)      # (dense rows are large: no second copy is held)
         return res
 
     @staticmethod

@@ -92,3 +92,13 @@ def test_scores_are_computed_once_in_each_mode(deferred):
     with torch.no_grad():
         out.token_nll(y, 0), out.materialize()
     assert (PlainNLL.calls, PlainDense.calls) == (2, 2)
+
+
+def test_one_copy_is_held_once_training_asks(deferred):
+    """A result with a history takes the place of the one without: dense rows are not held twice."""
+    out, y = deferred
+    with torch.no_grad():
+        scored = out.materialize()
+    trained = out.materialize()
+    dense = [t for t in out._nll_cache.values() if torch.is_tensor(t) and t.shape == scored.shape]
+    assert len(dense) == 1 and dense[0] is trained and out._dense is trained and trained is not scored
